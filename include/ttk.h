@@ -388,6 +388,93 @@ int ttk_softmax_fwd(const float* x, float* y, int64_t R, int64_t C, int log, voi
 int ttk_softmax_bwd(const float* y, const float* dy, float* dx, int accumulate, int64_t R,
                     int64_t C, int log, void* stream);
 
+/* ------------------------------- operators of a distilled student's training
+ * (no counterparts in the reference) */
+
+/* Scaled embedding: out[i,:] = scale * W[idx[i],:]; idx[i] = -1 (padding)
+ * gives a zero row. Any other id outside [0, V) sets bit 1 of the device
+ * status and counts as padding. W [V,D], out [N,D]. */
+int ttk_embedding_scaled_fwd(const float* W, const int64_t* idx, float* out, int64_t N, int64_t D,
+                             int64_t V, float scale, void* stream);
+/* Its gradient by sorted tokens: dW[v,:] = scale * sum of dout[i,:] over the
+ * positions i with idx[i] = v (zero rows for tokens that do not occur), or
+ * dW += the same with accumulate != 0. Padding and out-of-range ids add
+ * nothing. The summation order depends on the ids and on N and D alone: equal
+ * calls give equal bits. `workspace` (device, 16-byte aligned) must hold
+ * ttk_embedding_scaled_bwd_workspace_size(N, D, V) bytes; N and V below 2^31. */
+size_t ttk_embedding_scaled_bwd_workspace_size(int64_t N, int64_t D, int64_t V);
+int ttk_embedding_scaled_bwd(const float* dout, const int64_t* idx, float* dW, int accumulate,
+                             int64_t N, int64_t D, int64_t V, float scale, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
+/* Residual norm: the RMSNorm after a block, its gate, the residual scale, the
+ * residual add, and the RMSNorm before the next block.
+ *   rstd_post = (mean(b^2) + eps)^-1/2, h = residual_scale * x + g * (b * rstd_post * w_post)
+ *   rstd_next = (mean(h^2) + eps)^-1/2, y = h * rstd_next * w_next
+ * x, b, h, y [R,D]; w_post, w_next [D]; rstd_* [R] (saved for the backward).
+ * The gate g is one of: none (1), a scalar [1], per column [D], per row [R],
+ * per element [R,D]. w_next NULL leaves the second norm out (y and rstd_next
+ * unused). y_split (or NULL) receives the bf16x3 GEMM operand planes of y, bit
+ * for bit those of ttk_gemm_split(y, R, D, D, 0, 1, y_split): D a multiple of
+ * 32, bf16x3 precision. Outputs must not overlap inputs. */
+#define TTK_GATE_NONE 0
+#define TTK_GATE_SCALAR 1
+#define TTK_GATE_COLUMN 2
+#define TTK_GATE_ROW 3
+#define TTK_GATE_FULL 4
+int ttk_residual_norm_fwd(const float* x, const float* b, const float* w_post, const float* gate,
+                          int gate_kind, const float* w_next, float* h, float* y, float* rstd_post,
+                          float* rstd_next, void* y_split, int64_t R, int64_t D,
+                          float residual_scale, float eps, void* stream);
+/* Gradients for dh (of h, past the second norm; NULL: none) and dy (of y;
+ * NULL: none; one of the two is needed): dx, db [R,D], dw_post, dw_next [D]
+ * and dgate in the gate's shape (each of these three may be NULL). `accumulate`
+ * is a set of TTK_ACC_* bits: the outputs that are added to instead of
+ * written. h, w_next and rstd_next are read only with dy. Outputs must not
+ * overlap inputs. The sums over rows are taken in a fixed order. `workspace` (device, 16-byte aligned) must hold
+ * ttk_residual_norm_bwd_workspace_size(R, D) bytes. */
+#define TTK_ACC_DX 1
+#define TTK_ACC_DB 2
+#define TTK_ACC_DW 4
+#define TTK_ACC_DGATE 8
+size_t ttk_residual_norm_bwd_workspace_size(int64_t R, int64_t D);
+int ttk_residual_norm_bwd(const float* dh, const float* dy, const float* h, const float* b,
+                          const float* w_post, const float* gate, int gate_kind,
+                          const float* w_next, const float* rstd_post, const float* rstd_next,
+                          float* dx, float* db, float* dw_post, float* dw_next, float* dgate,
+                          int accumulate, int64_t R, int64_t D, float residual_scale,
+                          void* workspace, size_t workspace_bytes, void* stream);
+
+/* Distillation loss on a teacher's top logits. Per row i with student logits
+ * x = logits + i * ld (C classes) and the teacher's list (teacher_ids[i,k],
+ * teacher_logits[i,k]), k < K:
+ *   p = softmax(teacher_logits / T) over the list, q_T = softmax(x / T), q_1 = softmax(x)
+ *   KD = sum_k p_k (log p_k - log q_T[id_k]),  CE = -log q_1[targets[i]]
+ *   kd = grad_scale * sum_i w_i KD_i,  ce = grad_scale * sum_i w_i CE_i
+ *   loss[0..2] = { alpha T^2 kd + (1 - alpha) ce, kd, ce }
+ * and, when dlogits is not NULL, dlogits (row stride ldd) is the gradient of
+ * loss[0]. dlogits may be logits (with ldd = ld); columns past C are not
+ * touched. teacher_logits are of type teacher_type (TTK_F32, TTK_BF16 or
+ * TTK_F16).
+ *   - teacher_ids -1: no entry (a short list); a list without entries, or with
+ *     logits of -inf alone, gives no KD part; entries of one class add up
+ *   - targets NULL or targets[i] = -1: no CE part; row_weight NULL: all 1
+ *   - w_i = 0: the row is not read and its gradient is zero
+ *   - other ids out of range set bit 1 of the device status and are skipped
+ *   - logits of -inf are classes of probability 0; a teacher entry on one
+ *     makes the loss infinite; a row of -inf alone gives NaN, as softmax does
+ * K at most 1024. `workspace` (device, 16-byte aligned) must hold
+ * ttk_distill_loss_workspace_size(N) bytes. */
+#define TTK_F32 0
+#define TTK_BF16 1
+#define TTK_F16 2
+size_t ttk_distill_loss_workspace_size(int64_t N);
+int ttk_distill_loss(const float* logits, int64_t ld, const int32_t* teacher_ids,
+                     const void* teacher_logits, int teacher_type, int64_t K,
+                     const int64_t* targets, const float* row_weight, int64_t N, int64_t C,
+                     float alpha, float temperature, float grad_scale, float* loss, float* dlogits,
+                     int64_t ldd, void* workspace, size_t workspace_bytes, void* stream);
+
 /* --------------------------------------------------------------- optimizer */
 
 /* Sum of squares of a list of tensors, accumulated in fp64 into *acc

@@ -117,6 +117,15 @@ SIGS = {
     "ttk_axpy_dev": (I32, [P, P, P, I64, I32, P]),
     "ttk_softmax_fwd": (I32, [P, P, I64, I64, I32, P]),
     "ttk_softmax_bwd": (I32, [P, P, P, I32, I64, I64, I32, P]),
+    "ttk_embedding_scaled_fwd": (I32, [P, P, P, I64, I64, I64, F32, P]),
+    "ttk_embedding_scaled_bwd_workspace_size": (SZ, [I64, I64, I64]),
+    "ttk_embedding_scaled_bwd": (I32, [P, P, P, I32, I64, I64, I64, F32, P, SZ, P]),
+    "ttk_residual_norm_fwd": (I32, [P, P, P, P, I32] + [P] * 6 + [I64, I64, F32, F32, P]),
+    "ttk_residual_norm_bwd_workspace_size": (SZ, [I64, I64]),
+    "ttk_residual_norm_bwd": (I32, [P] * 6 + [I32] + [P] * 8 + [I32, I64, I64, F32, P, SZ, P]),
+    "ttk_distill_loss_workspace_size": (SZ, [I64]),
+    "ttk_distill_loss": (I32, [P, I64, P, P, I32, I64, P, P, I64, I64, F32, F32, F32, P, P, I64, P,
+                               SZ, P]),
     "ttk_sumsq_multi": (I32, [P, P, I32, P, P]),
     "ttk_adamw_multi": (I32, [P, P, P, P, P, I32, F32, F32, F32, F32, F32, I64, P, F32, F32, P]),
     "ttk_adamw_multi_sched": (I32, [P, P, P, P, P, I32, F32, F32, F32, F32, P, P, F32, F32, P]),

@@ -22,9 +22,11 @@ def _p(t):
     return None if t is None else t.data_ptr()
 
 
-def _chk(t, name):
-    if not (t.is_cuda and t.dtype == torch.float32 and t.is_contiguous()):
-        raise ValueError(f"{name}: expected a contiguous float32 CUDA tensor")
+def _chk(t, name, dtype=torch.float32, shape=None):
+    if not (t.is_cuda and t.dtype == dtype and t.is_contiguous()):
+        raise ValueError(f"{name}: expected a contiguous {str(dtype).split('.')[-1]} CUDA tensor")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name}: expected shape {list(shape)}, got {list(t.shape)}")
 
 
 def workspace(nbytes: int, device=None) -> torch.Tensor:
@@ -141,6 +143,146 @@ def embedding_bwd(dout, idx, dW):
     ws = workspace(call("ttk_embedding_bwd_workspace_size", N), dW.device)
     call("ttk_embedding_bwd", _p(dout), _p(idx), _p(dW), N, D, V, _p(ws), ws.numel(), _s())
     return dW
+
+
+def embedding_scaled_fwd(W, idx, scale=1.0):
+    """scale * W[idx] ([N, D]); idx -1 gives a zero row."""
+    _chk(W, "W")
+    _chk(idx, "idx", torch.int64)
+    V, D = W.shape
+    N = idx.numel()
+    out = torch.empty((N, D), dtype=torch.float32, device=W.device)
+    call("ttk_embedding_scaled_fwd", _p(W), _p(idx), _p(out), N, D, V, scale, _s())
+    return out
+
+
+def embedding_scaled_bwd(dout, idx, V, scale=1.0, dW=None, accumulate=False):
+    """Gradient of embedding_scaled_fwd for W [V, D], by sorted tokens: written
+    into dW (zero rows for tokens that do not occur) or, with accumulate,
+    added to it."""
+    _chk(dout, "dout")
+    _chk(idx, "idx", torch.int64)
+    N, D = dout.shape
+    if idx.numel() != N:
+        raise ValueError(f"idx: expected {N} ids, got {idx.numel()}")
+    if dW is None:
+        dW = (torch.zeros if accumulate else torch.empty)((V, D), dtype=torch.float32,
+                                                          device=dout.device)
+    _chk(dW, "dW", shape=(V, D))
+    ws = workspace(call("ttk_embedding_scaled_bwd_workspace_size", N, D, V), dout.device)
+    call("ttk_embedding_scaled_bwd", _p(dout), _p(idx), _p(dW), int(accumulate), N, D, V, scale,
+         _p(ws), ws.numel(), _s())
+    return dW
+
+
+def _gate_kind(gate, R, D):
+    """TTK_GATE_* of a gate tensor: None, [1], [D], [R, 1] or [R, D]."""
+    if gate is None:
+        return 0
+    _chk(gate, "gate")
+    shape = tuple(gate.shape)
+    if shape == (1,):
+        return 1
+    if shape == (D,):
+        return 2
+    if shape == (R, 1):
+        return 3
+    if shape == (R, D):
+        return 4
+    raise ValueError(f"gate: expected [1], [{D}], [{R}, 1] or [{R}, {D}], got {list(shape)}")
+
+
+def residual_norm_fwd(x, b, w_post, w_next=None, gate=None, residual_scale=1.0, eps=1e-5,
+                      planes=False):
+    """(h, y, rstd_post, rstd_next): h = residual_scale * x + gate * rmsnorm(b, w_post),
+    y = rmsnorm(h, w_next). Without w_next y and rstd_next are None. gate: None, [1], [D],
+    [R, 1] or [R, D]. With planes also the bf16x3 GEMM operand planes of y."""
+    R, D = x.shape
+    for t, name, shape in ((x, "x", (R, D)), (b, "b", (R, D)), (w_post, "w_post", (D,)),
+                           (w_next, "w_next", (D,))):
+        if t is not None:
+            _chk(t, name, shape=shape)
+    kind = _gate_kind(gate, R, D)
+    h = torch.empty_like(x)
+    rstd = torch.empty((2, R), dtype=torch.float32, device=x.device)
+    y = None if w_next is None else torch.empty_like(x)
+    split = workspace(call("ttk_gemm_split_bytes", 1, R, D), x.device) if planes else None
+    call("ttk_residual_norm_fwd", _p(x), _p(b), _p(w_post), _p(gate), kind, _p(w_next), _p(h),
+         _p(y), _p(rstd), rstd.data_ptr() + 4 * R, _p(split), R, D, residual_scale, eps, _s())
+    out = (h, y, rstd[0], None if w_next is None else rstd[1])
+    return out + (split,) if planes else out
+
+
+def residual_norm_bwd(dh, dy, h, b, w_post, w_next, rstd_post, rstd_next, gate=None,
+                      residual_scale=1.0, dx=None, db=None, dw_post=None, dw_next=None,
+                      dgate=None):
+    """(dx, db, dw_post, dw_next, dgate) of residual_norm_fwd; dh or dy may be None (no gradient
+    there). Output tensors that are given are added to; dgate is None without a gate, dw_next
+    without dy."""
+    R, D = b.shape
+    for t, name, shape in ((dh, "dh", (R, D)), (dy, "dy", (R, D)), (h, "h", (R, D)),
+                           (b, "b", (R, D)), (w_post, "w_post", (D,)), (w_next, "w_next", (D,)),
+                           (rstd_post, "rstd_post", (R,)), (rstd_next, "rstd_next", (R,)),
+                           (dx, "dx", (R, D)), (db, "db", (R, D)), (dw_post, "dw_post", (D,)),
+                           (dw_next, "dw_next", (D,)),
+                           (dgate, "dgate", None if gate is None else tuple(gate.shape))):
+        if t is not None:
+            _chk(t, name, shape=shape)
+    kind = _gate_kind(gate, R, D)
+    acc = (dx is not None) | (db is not None) << 1 | (dgate is not None) << 3
+    dx = torch.empty_like(b) if dx is None else dx
+    db = torch.empty_like(b) if db is None else db
+    # one flag covers both weights' gradients
+    acc |= (dw_post is not None or dw_next is not None) << 2
+    new_w = torch.zeros if acc & 4 else torch.empty
+    if dw_post is None:
+        dw_post = new_w(D, dtype=torch.float32, device=b.device)
+    if dw_next is None and dy is not None:
+        dw_next = new_w(D, dtype=torch.float32, device=b.device)
+    if dgate is None and gate is not None:
+        dgate = torch.empty_like(gate)
+    ws = workspace(call("ttk_residual_norm_bwd_workspace_size", R, D), b.device)
+    call("ttk_residual_norm_bwd", _p(dh), _p(dy), _p(h), _p(b), _p(w_post), _p(gate), kind,
+         _p(w_next), _p(rstd_post), _p(rstd_next), _p(dx), _p(db), _p(dw_post),
+         _p(dw_next) if dy is not None else None, _p(dgate), acc, R, D, residual_scale, _p(ws),
+         ws.numel(), _s())
+    return dx, db, dw_post, dw_next, dgate
+
+
+_TEACHER_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def distill_loss(logits, teacher_ids, teacher_logits, targets=None, alpha=1.0, temperature=1.0,
+                 row_weight=None, grad_scale=None, want_grad=True, dlogits=None):
+    """(loss, dlogits): loss [3] = {alpha T^2 kd + (1 - alpha) ce, kd, ce}, sums over the rows
+    times grad_scale (default 1 / N), kd against the teacher's top lists (ids [N, K] int32 with -1
+    for no entry, logits [N, K] fp32, bf16 or fp16) and ce against targets (int64, -1 for none).
+    logits [N, C] and dlogits may be views of wider rows (stride(1) = 1); dlogits may be logits."""
+    N, C = logits.shape
+    K = teacher_ids.shape[1]
+    for t, name in ((logits, "logits"), (dlogits, "dlogits")):
+        if t is not None and not (t.is_cuda and t.dtype == torch.float32 and
+                                  tuple(t.shape) == (N, C) and (t.stride(1) == 1 or C == 1) and
+                                  (t.stride(0) >= C or N <= 1)):
+            raise ValueError(f"{name}: expected float32 CUDA rows [{N}, {C}] of unit stride")
+    if teacher_logits.dtype not in _TEACHER_TYPES:
+        raise ValueError("teacher_logits: expected float32, bfloat16 or float16")
+    _chk(teacher_ids, "teacher_ids", torch.int32, (N, K))
+    _chk(teacher_logits, "teacher_logits", teacher_logits.dtype, (N, K))
+    if targets is not None:
+        _chk(targets, "targets", torch.int64, (N,))
+    if row_weight is not None:
+        _chk(row_weight, "row_weight", shape=(N,))
+    if want_grad and dlogits is None:
+        dlogits = torch.empty((N, C), dtype=torch.float32, device=logits.device)
+    loss = torch.empty(3, dtype=torch.float32, device=logits.device)
+    ws = workspace(call("ttk_distill_loss_workspace_size", N), logits.device)
+    call("ttk_distill_loss", _p(logits), max(logits.stride(0), C), _p(teacher_ids),
+         _p(teacher_logits), _TEACHER_TYPES[teacher_logits.dtype], K, _p(targets), _p(row_weight),
+         N, C, alpha, temperature, 1.0 / max(N, 1) if grad_scale is None else grad_scale, _p(loss),
+         _p(dlogits) if want_grad else None, max(dlogits.stride(0), C) if want_grad else 0, _p(ws),
+         ws.numel(), _s())
+    return loss, dlogits if want_grad else None
 
 
 def rope_fwd(x, cos, sin):
