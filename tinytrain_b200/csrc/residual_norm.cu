@@ -15,15 +15,19 @@
 //
 // Both directions are bound by HBM: 16 bytes per element forward (x, b in;
 // h, y out), 24 backward (dh, dy, h, b in; dx, db out), 4 or 8 more with a
-// gate per element. A row is spread over TPR threads that keep it in
-// registers from its one read to its writes, and the next row's loads are
-// issued before this row's sums, so a thread always has a row in flight.
+// gate per element. A row belongs to TPR threads (a slot of the block) that
+// keep it in registers from its one read to its writes. The rows come through
+// shared memory: one thread of the slot copies the slot's next rows with bulk
+// copies, as many ahead as the memory holds, so the reads go on while the
+// slot adds up, waits at its barrier and writes.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
 #include <algorithm>
+#include <atomic>
 #include <initializer_list>
 
+#include "pdl.cuh"
 #include "ttk_common.cuh"
 #include "ttk_internal.h"
 
@@ -133,25 +137,34 @@ struct Cols {
     }
 };
 
-// Sums of N values over the threads of a row. A row of one warp needs no
-// barrier; otherwise the warps meet in red, which the caller alternates
-// between two halves so that one barrier per sum is enough.
-constexpr int MAX_WARPS = 32;
+// Sums of N values over the threads of a row, and whether `ok` holds in all of
+// them. A row of one warp needs no barrier; otherwise the warps meet in red,
+// which the caller alternates between two halves so that one barrier per sum
+// is enough. Every thread of the slot gets here: its waits are bounded.
+constexpr int MAX_WARPS = 16;
 template <int N>
-__device__ __forceinline__ void row_sum(float (&v)[N], float* red, int tpr, bool one_warp) {
+__device__ __forceinline__ bool row_sum(float (&v)[N], float* red, int slot, int tpr, bool ok) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1)
 #pragma unroll
         for (int i = 0; i < N; ++i)
             v[i] += __shfl_xor_sync(~0u, v[i], o);
-    if (one_warp)
-        return;
-    const int warp = threadIdx.x >> 5, w0 = threadIdx.x / tpr * (tpr >> 5), nw = tpr >> 5;
+    if (tpr == 32)
+        return __all_sync(~0u, ok);
+    const int warp = threadIdx.x >> 5, w0 = slot * (tpr >> 5), nw = tpr >> 5;
     if ((threadIdx.x & 31) == 0)
 #pragma unroll
         for (int i = 0; i < N; ++i)
             red[i * MAX_WARPS + warp] = v[i];
-    __syncthreads();
+    uint32_t all;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "bar.red.and.pred q, %2, %3, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(all)
+        : "r"(static_cast<uint32_t>(ok)), "r"(1 + slot), "r"(tpr)
+        : "memory");
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         float s = 0.0f;
@@ -159,16 +172,111 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float* red, int tpr, bool
             s += red[i * MAX_WARPS + w0 + w];
         v[i] = s;
     }
+    return all != 0;
 }
 
+// A row of a tensor [R, D] as a bulk copy moves it: 16-byte pieces. `off` is
+// the row's start within its first piece, the copy covers elements [head,
+// tail) of the row. Pieces that the row shares with its neighbours are copied
+// whole; at the tensor's two ends, where there is no neighbour, the few
+// elements of such a piece are left to plain loads.
+struct Span {
+    const float* src;
+    int off, head, tail;
+    uint32_t bytes;
+};
+
+template <int VEC>
+__device__ __forceinline__ Span span_of(const float* base, int64_t row, int64_t R, int64_t D) {
+    const float* p = base + row * D;
+    if constexpr (VEC == 4)
+        return Span{p, 0, 0, static_cast<int>(D), static_cast<uint32_t>(D) * 4u};
+    Span s;
+    s.off = static_cast<int>((reinterpret_cast<uintptr_t>(p) & 15) >> 2);
+    s.head = -s.off;
+    if (s.off && row == 0)
+        s.head += 4;
+    s.tail = static_cast<int>((D + s.off + 3) / 4 * 4) - s.off;
+    if (s.tail > D && row == R - 1)
+        s.tail -= 4;
+    s.src = p + s.head;
+    s.bytes = s.tail > s.head ? static_cast<uint32_t>(s.tail - s.head) * 4u : 0u;
+    return s;
+}
+
+constexpr int MAX_STAGES = 4;
+constexpr int MAX_SLOTS = 8;
+
+// The slot's stages of NT rows (one per tensor; a null tensor is skipped and
+// reads as zeros), `pitch` floats each.
+template <int VEC, int NV, int NT>
+struct Feed {
+    static constexpr int E = VEC * NV;
+    const float* t[NT];
+    float* buf;  // [stages][NT][pitch]
+    uint64_t* bar;
+    int64_t R, D;
+    int pitch, stages;
+
+    __device__ __forceinline__ void issue(int stage, int64_t row) const {
+        uint32_t bytes = 0;
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+            if (t[i])
+                bytes += span_of<VEC>(t[i], row, R, D).bytes;
+        mbar_arrive_expect_tx(bar + stage, bytes);
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+            if (t[i]) {
+                const Span s = span_of<VEC>(t[i], row, R, D);
+                if (s.bytes)
+                    bulk_load(buf + (stage * NT + i) * pitch + s.off + s.head, s.src, s.bytes,
+                              bar + stage);
+            }
+    }
+    __device__ __forceinline__ void read(float (&v)[E], int i, int stage, int64_t row,
+                                         const Cols<VEC, NV>& cols) const {
+        const float* b = buf + (stage * NT + i) * pitch;
+        if (VEC == 4 || !t[i])
+            return cols.load(v, b, t[i] != nullptr);
+        const Span s = span_of<VEC>(t[i], row, R, D);
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            v[j] = !cols.in[j] ? 0.0f
+                   : cols.c[j] >= s.head && cols.c[j] < s.tail ? b[s.off + cols.c[j]]
+                                                               : t[i][row * D + cols.c[j]];
+    }
+};
+
 template <int VEC, int NV, bool FULL>
-__global__ void __launch_bounds__(512) fwd_rows_kernel(const Fwd a, int tpr) {
-    constexpr int E = VEC * NV;
+__global__ void __launch_bounds__(512) fwd_rows_kernel(const Fwd a, int tpr, int pitch, int stages) {
+    constexpr int E = VEC * NV, NT = FULL ? 3 : 2;
+    extern __shared__ __align__(16) float smem[];
     __shared__ float red[2][MAX_WARPS];
+    __shared__ __align__(8) uint64_t bars[MAX_SLOTS * MAX_STAGES];
     const int slot = threadIdx.x / tpr, slots = blockDim.x / tpr;
-    const bool one_warp = tpr == 32;
+    const bool lead = threadIdx.x == slot * tpr;
     const int64_t D = a.D;
     const Cols<VEC, NV> cols(threadIdx.x - slot * tpr, tpr, D);
+    Feed<VEC, NV, NT> feed;
+    feed.t[0] = a.b, feed.t[1] = a.x;
+    if constexpr (FULL)
+        feed.t[2] = a.g.p;
+    feed.buf = smem + static_cast<int64_t>(slot) * stages * NT * pitch;
+    feed.bar = bars + slot * MAX_STAGES;
+    feed.R = a.R, feed.D = D, feed.pitch = pitch, feed.stages = stages;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * slots;
+    int64_t row = static_cast<int64_t>(blockIdx.x) * slots + slot;
+    if (lead) {
+        for (int s = 0; s < stages; ++s)
+            mbar_init(feed.bar + s, 1);
+        fence_barrier_init();
+    }
+    __syncthreads();
+    grid_wait();
+    if (lead)
+        for (int s = 0; s < stages && row + s * step < a.R; ++s)
+            feed.issue(s, row + s * step);
     const float inv = 1.0f / static_cast<float>(D);
     float w1[E], w2[E];  // w1 with a gate per column folded in
     cols.load(w1, a.w1, true);
@@ -180,83 +288,103 @@ __global__ void __launch_bounds__(512) fwd_rows_kernel(const Fwd a, int tpr) {
         for (int i = 0; i < E; ++i)
             w1[i] *= g[i];
     }
-    const int64_t step = static_cast<int64_t>(gridDim.x) * slots;
-    float x[E], b[E], g[FULL ? E : 1];
-    auto fetch = [&](int64_t row, float (&xv)[E], float (&bv)[E], float (&gv)[FULL ? E : 1]) {
-        const bool ok = row < a.R;
-        cols.load(bv, a.b + row * D, ok);
-        cols.load(xv, a.x + row * D, ok);
+    int stage = 0;
+    uint32_t phase = 0;
+    for (; row < a.R; row += step) {
+        const float gr = a.g.of_row(row);
+        bool ok = mbar_wait(feed.bar + stage, phase, 90);
+        float x[E], b[E], g[FULL ? E : 1];
+        feed.read(b, 0, stage, row, cols);
+        feed.read(x, 1, stage, row, cols);
         if constexpr (FULL)
-            cols.load(gv, a.g.p + row * D, ok);
-    };
-    int64_t row = static_cast<int64_t>(blockIdx.x) * slots + slot;
-    fetch(row, x, b, g);
-    for (int64_t base = static_cast<int64_t>(blockIdx.x) * slots; base < a.R;
-         base += step, row += step) {
-        const bool ok = row < a.R;
-        float nx[E], nb[E], ng[FULL ? E : 1];
-        fetch(row + step, nx, nb, ng);
+            feed.read(g, 2, stage, row, cols);
         float s[1] = {0.0f};
 #pragma unroll
         for (int i = 0; i < E; ++i)
             s[0] += b[i] * b[i];
-        row_sum(s, red[0], tpr, one_warp);
+        ok = row_sum(s, red[0], slot, tpr, ok);
+        if (!ok) {
+            // a copy did not arrive: the slot stops once its copies have ended
+            if (lead)
+                for (int64_t i = 0; i < stages && row + i * step < a.R; ++i) {
+                    mbar_wait(feed.bar + stage, phase, 91);
+                    if (++stage == stages)
+                        stage = 0, phase ^= 1;
+                }
+            break;
+        }
+        if (lead && row + stages * step < a.R) {  // every thread has read the stage
+            fence_async_smem();
+            feed.issue(stage, row + stages * step);
+        }
+        if (++stage == stages)
+            stage = 0, phase ^= 1;
         const float r1 = 1.0f / sqrtf(s[0] * inv + a.eps);
-        const float k = ok ? r1 * a.g.of_row(row) : 0.0f;
-        float h[E];
+        const float k = r1 * gr;
         s[0] = 0.0f;
 #pragma unroll
         for (int i = 0; i < E; ++i) {
             float u = b[i] * k * w1[i];
             if constexpr (FULL)
                 u *= g[i];
-            h[i] = a.alpha * x[i] + u;
-            s[0] += h[i] * h[i];
+            x[i] = a.alpha * x[i] + u;  // h
+            s[0] += x[i] * x[i];
         }
-        row_sum(s, red[1], tpr, one_warp);
+        cols.store(a.h + row * D, x);
+        row_sum(s, red[1], slot, tpr, true);
         const float r2 = 1.0f / sqrtf(s[0] * inv + a.eps);
-        if (ok) {
-            cols.store(a.h + row * D, h);
-            if (threadIdx.x == slot * tpr) {
-                a.r1[row] = r1;
-                if (a.w2)
-                    a.r2[row] = r2;
-            }
-            if (a.w2) {
-#pragma unroll
-                for (int i = 0; i < E; ++i)
-                    h[i] *= r2 * w2[i];
-                cols.store(a.y + row * D, h);
-                if (a.split)
-                    cols.store_split(a.split + row * D, a.R * D, h);
-            }
+        if (lead) {
+            a.r1[row] = r1;
+            if (a.w2)
+                a.r2[row] = r2;
         }
-#pragma unroll
-        for (int i = 0; i < E; ++i)
-            x[i] = nx[i], b[i] = nb[i];
-        if constexpr (FULL)
+        if (a.w2) {
 #pragma unroll
             for (int i = 0; i < E; ++i)
-                g[i] = ng[i];
+                x[i] *= r2 * w2[i];
+            cols.store(a.y + row * D, x);
+            if (a.split)
+                cols.store_split(a.split + row * D, a.R * D, x);
+        }
     }
 }
 
 template <int VEC, int NV, bool FULL>
-__global__ void __launch_bounds__(512) bwd_rows_kernel(const Bwd a, int tpr) {
-    constexpr int E = VEC * NV;
-    extern __shared__ float sums[];  // [slots - 1][2][D]: the other slots' column sums
+__global__ void __launch_bounds__(512) bwd_rows_kernel(const Bwd a, int tpr, int pitch, int stages) {
+    constexpr int E = VEC * NV, NT = FULL ? 5 : 4;
+    extern __shared__ __align__(16) float smem[];
     __shared__ float red[2][3 * MAX_WARPS];
-    __shared__ double s_g[MAX_WARPS];
+    __shared__ double s_g[MAX_SLOTS];
+    __shared__ __align__(8) uint64_t bars[MAX_SLOTS * MAX_STAGES];
     const int slot = threadIdx.x / tpr, slots = blockDim.x / tpr;
-    const bool one_warp = tpr == 32, lead = threadIdx.x == slot * tpr;
+    const bool lead = threadIdx.x == slot * tpr;
     const int64_t D = a.D;
     const Cols<VEC, NV> cols(threadIdx.x - slot * tpr, tpr, D);
+    const bool need_dy = a.dy != nullptr;
+    Feed<VEC, NV, NT> feed;
+    feed.t[0] = a.dy, feed.t[1] = need_dy ? a.h : nullptr, feed.t[2] = a.dh, feed.t[3] = a.b;
+    if constexpr (FULL)
+        feed.t[4] = a.g.p;
+    feed.buf = smem + static_cast<int64_t>(slot) * stages * NT * pitch;
+    feed.bar = bars + slot * MAX_STAGES;
+    feed.R = a.R, feed.D = D, feed.pitch = pitch, feed.stages = stages;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * slots;
+    int64_t row = static_cast<int64_t>(blockIdx.x) * slots + slot;
+    if (lead) {
+        for (int s = 0; s < stages; ++s)
+            mbar_init(feed.bar + s, 1);
+        fence_barrier_init();
+    }
+    __syncthreads();
+    grid_wait();
+    if (lead)
+        for (int s = 0; s < stages && row + s * step < a.R; ++s)
+            feed.issue(s, row + s * step);
     const float inv = 1.0f / static_cast<float>(D);
-    const bool column = a.g.kind == TTK_GATE_COLUMN, need_dy = a.dy != nullptr;
     float w1[E], w2[E];  // w1 with a gate per column folded in
     cols.load(w1, a.w1, true);
     cols.load(w2, a.w2, need_dy);
-    if (column) {
+    if (a.g.kind == TTK_GATE_COLUMN) {
         float g[E];
         cols.load(g, a.g.p, true);
 #pragma unroll
@@ -268,111 +396,107 @@ __global__ void __launch_bounds__(512) bwd_rows_kernel(const Bwd a, int tpr) {
     for (int i = 0; i < E; ++i)
         s1[i] = s2[i] = 0.0f;
     double gsum = 0.0;
-    struct Row {
-        float dh[E], dy[E], h[E], b[E], g[FULL ? E : 1];
-        float r1, r2, gr;
-    };
-    auto fetch = [&](int64_t row, Row& v) {
-        const bool ok = row < a.R;
-        cols.load(v.dy, a.dy + row * D, ok && need_dy);
-        cols.load(v.h, a.h + row * D, ok && need_dy);
-        cols.load(v.dh, a.dh + row * D, ok && a.dh);
-        cols.load(v.b, a.b + row * D, ok);
+    int stage = 0, parity = 0;
+    uint32_t phase = 0;
+    for (; row < a.R; row += step, parity ^= 1) {
+        const float r1 = a.r1[row], r2 = need_dy ? a.r2[row] : 0.0f, gr = a.g.of_row(row);
+        bool ok = mbar_wait(feed.bar + stage, phase, 92);
+        float dy[E], h[E], dh[E], b[E], g[FULL ? E : 1];
+        feed.read(dy, 0, stage, row, cols);
+        feed.read(h, 1, stage, row, cols);
+        feed.read(dh, 2, stage, row, cols);
+        feed.read(b, 3, stage, row, cols);
         if constexpr (FULL)
-            cols.load(v.g, a.g.p + row * D, ok);
-        v.r1 = ok ? a.r1[row] : 0.0f;
-        v.r2 = ok && need_dy ? a.r2[row] : 0.0f;
-        v.gr = ok ? a.g.of_row(row) : 0.0f;
-    };
-    const int64_t step = static_cast<int64_t>(gridDim.x) * slots;
-    int64_t row = static_cast<int64_t>(blockIdx.x) * slots + slot;
-    int parity = 0;
-    Row v;
-    fetch(row, v);
-    for (int64_t base = static_cast<int64_t>(blockIdx.x) * slots; base < a.R;
-         base += step, row += step, parity ^= 1) {
-        const bool ok = row < a.R;
-        Row n;
-        fetch(row + step, n);
+            feed.read(g, 4, stage, row, cols);
         float s[3] = {0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-            const float e = v.dy[i] * w2[i];
-            float c = w1[i] * v.b[i];
+            const float e = dy[i] * w2[i];
+            float c = w1[i] * b[i];
             if constexpr (FULL)
-                c *= v.g[i];
-            s[0] += e * v.h[i];
-            s[1] += (v.dh[i] + v.r2 * e) * c;
-            s[2] += v.h[i] * c;
+                c *= g[i];
+            s[0] += e * h[i];
+            s[1] += (dh[i] + r2 * e) * c;
+            s[2] += h[i] * c;
         }
-        row_sum(s, red[parity], tpr, one_warp);
-        const float k2 = v.r2 * v.r2 * v.r2 * inv * s[0];
-        const float dot = s[1] - k2 * s[2];  // sum(f b) without a gate of the whole row
-        const float k1 = v.r1 * v.r1 * v.r1 * inv * dot * v.gr, r1g = v.r1 * v.gr;
-        if (ok) {
-            float dx[E], db[E];
-            [[maybe_unused]] float dg[FULL ? E : 1];
-#pragma unroll
-            for (int i = 0; i < E; ++i) {
-                const float H = v.dh[i] + v.r2 * (v.dy[i] * w2[i]) - v.h[i] * k2;
-                float f = H * w1[i], hb = H * v.b[i] * r1g;
-                if constexpr (FULL) {
-                    dg[i] = hb * w1[i];
-                    f *= v.g[i];
-                    hb *= v.g[i];
+        ok = row_sum(s, red[parity], slot, tpr, ok);
+        if (!ok) {
+            // a copy did not arrive: the slot stops once its copies have ended
+            if (lead)
+                for (int64_t i = 0; i < stages && row + i * step < a.R; ++i) {
+                    mbar_wait(feed.bar + stage, phase, 93);
+                    if (++stage == stages)
+                        stage = 0, phase ^= 1;
                 }
-                dx[i] = a.alpha * H;
-                db[i] = r1g * f - v.b[i] * k1;
-                s1[i] += hb;
-                s2[i] += v.dy[i] * v.h[i] * v.r2;
-            }
-            cols.add_store(a.dx + row * D, dx, a.acc & TTK_ACC_DX);
-            cols.add_store(a.db + row * D, db, a.acc & TTK_ACC_DB);
-            if constexpr (FULL)
-                if (a.dgate)
-                    cols.add_store(a.dgate + row * D, dg, a.acc & TTK_ACC_DGATE);
-            if (lead) {
-                const float d = v.r1 * dot;
-                if (a.g.kind == TTK_GATE_ROW && a.dgate)
-                    a.dgate[row] = (a.acc & TTK_ACC_DGATE) ? a.dgate[row] + d : d;
-                gsum += static_cast<double>(d);
-            }
+            break;
         }
-        v = n;
+        if (lead && row + stages * step < a.R) {  // every thread has read the stage
+            fence_async_smem();
+            feed.issue(stage, row + stages * step);
+        }
+        if (++stage == stages)
+            stage = 0, phase ^= 1;
+        const float k2 = r2 * r2 * r2 * inv * s[0];
+        const float dot = s[1] - k2 * s[2];  // sum(f b) without a gate of the whole row
+        const float k1 = r1 * r1 * r1 * inv * dot * gr, r1g = r1 * gr;
+        float dx[E], db[E];
+        [[maybe_unused]] float dg[FULL ? E : 1];
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const float H = dh[i] + r2 * (dy[i] * w2[i]) - h[i] * k2;
+            float f = H * w1[i], hb = H * b[i] * r1g;
+            if constexpr (FULL) {
+                dg[i] = hb * w1[i];
+                f *= g[i];
+                hb *= g[i];
+            }
+            dx[i] = a.alpha * H;
+            db[i] = r1g * f - b[i] * k1;
+            s1[i] += hb;
+            s2[i] += dy[i] * h[i] * r2;
+        }
+        cols.add_store(a.dx + row * D, dx, a.acc & TTK_ACC_DX);
+        cols.add_store(a.db + row * D, db, a.acc & TTK_ACC_DB);
+        if constexpr (FULL)
+            if (a.dgate)
+                cols.add_store(a.dgate + row * D, dg, a.acc & TTK_ACC_DGATE);
+        if (lead) {
+            const float d = r1 * dot;
+            if (a.g.kind == TTK_GATE_ROW && a.dgate)
+                a.dgate[row] = (a.acc & TTK_ACC_DGATE) ? a.dgate[row] + d : d;
+            gsum += static_cast<double>(d);
+        }
     }
-    // the block's rows, slot by slot
+    // the block's rows, slot by slot, through the stages' memory
     if (slots > 1) {
+        __syncthreads();
         if (slot) {
-            cols.store(sums + (2 * slot - 2) * D, s1);
-            cols.store(sums + (2 * slot - 1) * D, s2);
+            cols.store(smem + (2 * slot - 2) * D, s1);
+            cols.store(smem + (2 * slot - 1) * D, s2);
         }
+        if (lead)
+            s_g[slot] = gsum;
         __syncthreads();
         if (slot == 0)
             for (int q = 1; q < slots; ++q) {
                 float o[E];
-                cols.load(o, sums + (2 * q - 2) * D, true);
+                cols.load(o, smem + (2 * q - 2) * D, true);
 #pragma unroll
                 for (int i = 0; i < E; ++i)
                     s1[i] += o[i];
-                cols.load(o, sums + (2 * q - 1) * D, true);
+                cols.load(o, smem + (2 * q - 1) * D, true);
 #pragma unroll
                 for (int i = 0; i < E; ++i)
                     s2[i] += o[i];
+                if (lead)
+                    gsum += s_g[q];
             }
     }
     if (slot == 0) {
         cols.store(a.part1 + blockIdx.x * D, s1);
         cols.store(a.part2 + blockIdx.x * D, s2);
-    }
-    if (a.g.kind == TTK_GATE_SCALAR) {
         if (lead)
-            s_g[slot] = gsum;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            for (int q = 1; q < slots; ++q)
-                gsum += s_g[q];
             a.partg[blockIdx.x] = gsum;
-        }
     }
 }
 
@@ -382,13 +506,14 @@ constexpr int WIDE_THREADS = 512;
 
 __global__ void __launch_bounds__(WIDE_THREADS) fwd_wide_kernel(const Fwd a) {
     __shared__ float red[2][MAX_WARPS];
+    grid_wait();
     const int64_t D = a.D;
     for (int64_t row = blockIdx.x; row < a.R; row += gridDim.x) {
         const int64_t o = row * D;
         float s[1] = {0.0f};
         for (int64_t c = threadIdx.x; c < D; c += WIDE_THREADS)
             s[0] += a.b[o + c] * a.b[o + c];
-        row_sum(s, red[0], WIDE_THREADS, false);
+        row_sum(s, red[0], 0, WIDE_THREADS, true);
         const float r1 = 1.0f / sqrtf(s[0] / static_cast<float>(D) + a.eps);
         s[0] = 0.0f;
         for (int64_t c = threadIdx.x; c < D; c += WIDE_THREADS) {
@@ -396,7 +521,7 @@ __global__ void __launch_bounds__(WIDE_THREADS) fwd_wide_kernel(const Fwd a) {
             a.h[o + c] = h;
             s[0] += h * h;
         }
-        row_sum(s, red[1], WIDE_THREADS, false);
+        row_sum(s, red[1], 0, WIDE_THREADS, true);
         const float r2 = 1.0f / sqrtf(s[0] / static_cast<float>(D) + a.eps);
         if (threadIdx.x == 0) {
             a.r1[row] = r1;
@@ -421,6 +546,7 @@ __global__ void __launch_bounds__(WIDE_THREADS) fwd_wide_kernel(const Fwd a) {
 // writes its own columns only).
 __global__ void __launch_bounds__(WIDE_THREADS) bwd_wide_kernel(const Bwd a) {
     __shared__ float red[2][3 * MAX_WARPS];
+    grid_wait();
     const int64_t D = a.D;
     float* p1 = a.part1 + blockIdx.x * D;
     float* p2 = a.part2 + blockIdx.x * D;
@@ -438,7 +564,7 @@ __global__ void __launch_bounds__(WIDE_THREADS) bwd_wide_kernel(const Bwd a) {
             s[1] += ((a.dh ? a.dh[o + c] : 0.0f) + r2 * e) * k;
             s[2] += h * k;
         }
-        row_sum(s, red[parity], WIDE_THREADS, false);
+        row_sum(s, red[parity], 0, WIDE_THREADS, true);
         const float k2 = r2 * r2 * r2 / static_cast<float>(D) * s[0];
         const float dot = s[1] - k2 * s[2];
         const float k1 = r1 * r1 * r1 / static_cast<float>(D) * dot * gr;
@@ -468,9 +594,9 @@ __global__ void __launch_bounds__(WIDE_THREADS) bwd_wide_kernel(const Bwd a) {
 }
 
 // Column sums of the nb partial rows into the weights' and the gate's
-// gradients: 32 columns a block, warp w adds rows w, w + 16, ... and the
+// gradients: 32 columns a block, warp w adds rows w, w + 32, ... and the
 // warps' sums are added in order.
-constexpr int FIN_WARPS = 16;
+constexpr int FIN_WARPS = 32;
 __global__ void __launch_bounds__(32 * FIN_WARPS) finish_kernel(const Bwd a, int64_t nb, float* dw1,
                                                                 float* dw2) {
     __shared__ float red[2][FIN_WARPS][32];
@@ -478,8 +604,9 @@ __global__ void __launch_bounds__(32 * FIN_WARPS) finish_kernel(const Bwd a, int
     const bool accw = a.acc & TTK_ACC_DW, accg = a.acc & TTK_ACC_DGATE;
     const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
     float s1 = 0.0f, s2 = 0.0f;
+    grid_wait();
     if (c < a.D) {
-#pragma unroll 4
+#pragma unroll 8
         for (int64_t i = warp; i < nb; i += FIN_WARPS) {
             s1 += a.part1[i * a.D + c];
             s2 += a.part2[i * a.D + c];
@@ -528,46 +655,84 @@ bool aligned16(std::initializer_list<const void*> ps) {
     return true;
 }
 
-// Blocks of `kernel` that are resident at once on the current device.
-template <class Kernel>
-int64_t resident(Kernel kernel, int threads, size_t smem) {
-    int dev = 0, sms = 0, per = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess ||
-        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-        sms = 148;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, threads, smem) != cudaSuccess ||
-        per <= 0) {
-        cudaGetLastError();
-        per = 1;
-    }
-    return static_cast<int64_t>(sms) * per;
+// The partial sums' places in the workspace, rows first (stored as float4).
+void partials(Bwd& a, int64_t nb, void* ws) {
+    a.part1 = static_cast<float*>(ws);
+    a.part2 = a.part1 + nb * a.D;
+    a.partg = reinterpret_cast<double*>(a.part2 + nb * a.D);  // after 2 nb D floats
 }
 
 constexpr int64_t MAX_ROW = 8192;     // widest row kept in registers
 constexpr int64_t MAX_BLOCKS = 2048;  // partial rows of the backward
+constexpr int SMEM_SM = 224 * 1024;   // shared memory of an SM for its blocks' stages
 
-template <int VEC, int NV, bool FULL>
-int run_fwd(const Fwd& a, cudaStream_t st) {
-    const int tpr = row_threads(a.D, VEC, NV), slots = std::max(1, 256 / tpr);
-    const int threads = tpr * slots;
-    const int64_t blocks = std::min((a.R + slots - 1) / slots,
-                                    resident(fwd_rows_kernel<VEC, NV, FULL>, threads, 0));
-    fwd_rows_kernel<VEC, NV, FULL><<<static_cast<int>(blocks), threads, 0, st>>>(a, tpr);
-    return check_launch("residual_norm_fwd");
+// Launch shape of a rows kernel: slots of TPR threads, whole rows each, up to
+// 256 threads a block; as many blocks as the registers let an SM hold, and
+// the shared memory left to each of them spent on stages.
+struct Shape {
+    int tpr, slots, threads, pitch, stages;
+    size_t smem;
+    int64_t resident;  // blocks
+};
+
+template <auto kernel>
+Shape shape_of(int64_t R, int64_t D, int vec, int nv, int tensors) {
+    Shape s;
+    s.tpr = row_threads(D, vec, nv);
+    s.slots = std::max(1, std::min(MAX_SLOTS, 256 / s.tpr));
+    s.threads = s.tpr * s.slots;
+    s.pitch = static_cast<int>(vec == 4 ? D : (D + 9) / 4 * 4);  // up to 3 floats at either end
+    // {SMs, blocks per SM} by device and block size, asked for once
+    constexpr int kDevs = 16;
+    static std::atomic<int> cache[kDevs][17];
+    int dev = 0, sms = 0, per = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev >= kDevs)
+        dev = 0;
+    std::atomic<int>& c = cache[dev][s.threads / 32];
+    const int known = c.load(std::memory_order_relaxed);
+    if (known) {
+        sms = known >> 8, per = known & 255;
+    } else {
+        if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+            sms = 148;
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_SM);
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, s.threads, 0) !=
+                cudaSuccess ||
+            per <= 0)
+            per = 1;
+        cudaGetLastError();
+        c.store(sms << 8 | per, std::memory_order_relaxed);
+    }
+    const size_t stage = static_cast<size_t>(s.slots) * tensors * s.pitch * sizeof(float);
+    const int64_t rows = (R + static_cast<int64_t>(sms) * per * s.slots - 1) /
+                         (static_cast<int64_t>(sms) * per * s.slots);  // per slot
+    const int64_t room = SMEM_SM / per > 2048 ? (SMEM_SM / per - 2048) / static_cast<int64_t>(stage) : 0;
+    s.stages = static_cast<int>(
+        std::max<int64_t>(1, std::min<int64_t>({room, rows, static_cast<int64_t>(MAX_STAGES)})));
+    s.smem = stage * s.stages;
+    while (per > 1 && per * (s.smem + 2048) > SMEM_SM)
+        --per;
+    s.resident = static_cast<int64_t>(sms) * per;
+    return s;
 }
 
 template <int VEC, int NV, bool FULL>
-int run_bwd(const Bwd& a, int64_t* nb, cudaStream_t st) {
-    const int tpr = row_threads(a.D, VEC, NV), slots = std::max(1, 256 / tpr);
-    const int threads = tpr * slots;
-    const size_t smem = static_cast<size_t>(slots - 1) * 2 * a.D * sizeof(float);
-    if (*nb == 0) {  // ask for the blocks alone
-        *nb = std::min({(a.R + slots - 1) / slots, MAX_BLOCKS,
-                        resident(bwd_rows_kernel<VEC, NV, FULL>, threads, smem)});
-        return TTK_OK;
-    }
-    bwd_rows_kernel<VEC, NV, FULL><<<static_cast<int>(*nb), threads, smem, st>>>(a, tpr);
-    return check_launch("residual_norm_bwd");
+int run_fwd(const Fwd& a, cudaStream_t st) {
+    const Shape s = shape_of<fwd_rows_kernel<VEC, NV, FULL>>(a.R, a.D, VEC, NV, FULL ? 3 : 2);
+    const int64_t blocks = std::min((a.R + s.slots - 1) / s.slots, s.resident);
+    return launch_pdl("residual_norm_fwd", fwd_rows_kernel<VEC, NV, FULL>,
+                      dim3(static_cast<unsigned>(blocks)), s.threads, s.smem, st, a, s.tpr, s.pitch,
+                      s.stages);
+}
+
+template <int VEC, int NV, bool FULL>
+int run_bwd(Bwd& a, int64_t* nb, void* ws, cudaStream_t st) {
+    const Shape s = shape_of<bwd_rows_kernel<VEC, NV, FULL>>(a.R, a.D, VEC, NV, FULL ? 5 : 4);
+    *nb = std::min({(a.R + s.slots - 1) / s.slots, MAX_BLOCKS, s.resident});
+    partials(a, *nb, ws);
+    return launch_pdl("residual_norm_bwd", bwd_rows_kernel<VEC, NV, FULL>,
+                      dim3(static_cast<unsigned>(*nb)), s.threads, s.smem, st, a, s.tpr, s.pitch,
+                      s.stages);
 }
 
 int dispatch_fwd(const Fwd& a, bool vec, cudaStream_t st) {
@@ -582,24 +747,22 @@ int dispatch_fwd(const Fwd& a, bool vec, cudaStream_t st) {
     return full ? run_fwd<1, 16, true>(a, st) : run_fwd<1, 16, false>(a, st);
 }
 
-int dispatch_bwd(const Bwd& a, bool vec, int64_t* nb, cudaStream_t st) {
+int dispatch_bwd(Bwd& a, bool vec, int64_t* nb, void* ws, cudaStream_t st) {
     if (a.D > MAX_ROW) {
-        if (*nb == 0) {
-            *nb = std::min<int64_t>(a.R, 296);
-            return TTK_OK;
-        }
-        bwd_wide_kernel<<<static_cast<int>(*nb), WIDE_THREADS, 0, st>>>(a);
-        return check_launch("residual_norm_bwd");
+        *nb = std::min<int64_t>(a.R, 296);
+        partials(a, *nb, ws);
+        return launch_pdl("residual_norm_bwd", bwd_wide_kernel, dim3(static_cast<unsigned>(*nb)),
+                          WIDE_THREADS, 0, st, a);
     }
     const bool full = a.g.kind == TTK_GATE_FULL;
     if (vec) {
         if (a.D <= 4096)
-            return full ? run_bwd<4, 2, true>(a, nb, st) : run_bwd<4, 2, false>(a, nb, st);
-        return full ? run_bwd<4, 4, true>(a, nb, st) : run_bwd<4, 4, false>(a, nb, st);
+            return full ? run_bwd<4, 2, true>(a, nb, ws, st) : run_bwd<4, 2, false>(a, nb, ws, st);
+        return full ? run_bwd<4, 4, true>(a, nb, ws, st) : run_bwd<4, 4, false>(a, nb, ws, st);
     }
     if (a.D <= 4096)
-        return full ? run_bwd<1, 8, true>(a, nb, st) : run_bwd<1, 8, false>(a, nb, st);
-    return full ? run_bwd<1, 16, true>(a, nb, st) : run_bwd<1, 16, false>(a, nb, st);
+        return full ? run_bwd<1, 8, true>(a, nb, ws, st) : run_bwd<1, 8, false>(a, nb, ws, st);
+    return full ? run_bwd<1, 16, true>(a, nb, ws, st) : run_bwd<1, 16, false>(a, nb, ws, st);
 }
 
 }  // namespace resnorm
@@ -643,10 +806,10 @@ int ttk_residual_norm_fwd(const float* x, const float* b, const float* w_post, c
         vec = vec && aligned16({gate});
     const Fwd a{x, b, w_post, Gate{gate, gate_kind}, w_next, h, y, rstd_post, rstd_next,
                 static_cast<__nv_bfloat16*>(y_split), R, D, residual_scale, eps};
-    if (D > MAX_ROW) {
-        fwd_wide_kernel<<<grid_for(R, 1, 148 * 4), WIDE_THREADS, 0, st>>>(a);
-        return check_launch("residual_norm_fwd");
-    }
+    if (D > MAX_ROW)
+        return launch_pdl("residual_norm_fwd", fwd_wide_kernel,
+                          dim3(static_cast<unsigned>(grid_for(R, 1, 148 * 4))), WIDE_THREADS, 0, st,
+                          a);
     return dispatch_fwd(a, vec, st);
 }
 
@@ -687,19 +850,12 @@ int ttk_residual_norm_bwd(const float* dh, const float* dy, const float* h, cons
             vec = vec && aligned16({gate});
         if (gate_kind == TTK_GATE_FULL)
             vec = vec && aligned16({gate, dgate});
-        int rc = dispatch_bwd(a, vec, &nb, st);
-        if (rc)
-            return rc;
-        a.part1 = static_cast<float*>(workspace);  // rows first: they are stored as float4
-        a.part2 = a.part1 + nb * D;
-        a.partg = reinterpret_cast<double*>(a.part2 + nb * D);  // 2 nb D floats: 8-byte aligned
-        rc = dispatch_bwd(a, vec, &nb, st);
-        if (rc)
+        if (int rc = dispatch_bwd(a, vec, &nb, workspace, st))
             return rc;
     }
-    finish_kernel<<<static_cast<int>((D + 31) / 32), 32 * FIN_WARPS, 0, st>>>(a, nb, dw_post,
-                                                                              dw_next);
-    return check_launch("residual_norm_bwd sums");
+    return launch_pdl("residual_norm_bwd sums", finish_kernel,
+                      dim3(static_cast<unsigned>((D + 31) / 32)), 32 * FIN_WARPS, 0, st, a, nb,
+                      dw_post, dw_next);
 }
 
 }  // extern "C"
