@@ -463,7 +463,7 @@ int ttk_residual_norm_bwd(const float* dh, const float* dy, const float* h, cons
  *   - other ids out of range set bit 1 of the device status and are skipped
  *   - logits of -inf are classes of probability 0; a teacher entry on one
  *     makes the loss infinite; a row of -inf alone gives NaN, as softmax does
- * K at most 1024. `workspace` (device, 16-byte aligned) must hold
+ * K at most 1024, C at most 2^30. `workspace` (device, 16-byte aligned) holds
  * ttk_distill_loss_workspace_size(N) bytes. */
 #define TTK_F32 0
 #define TTK_BF16 1

@@ -6,10 +6,18 @@
 //   KD = sum_k p_k (log p_k - log q_T[id_k]),   CE = -log q_1[target]
 //   L  = grad_scale * sum_rows w (alpha T^2 KD + (1 - alpha) CE)
 //   dx = grad_scale * w (alpha T (q_T - P) + (1 - alpha)(q_1 - onehot))
-// where P spreads p over the classes. One block per row: a first pass keeps a
-// running maximum and the running sums of exp(x - m) and exp((x - m) / T); a
-// second writes the gradient without the teacher's and the label's terms; the
-// few listed classes are then written once more with them.
+// where P spreads p over the classes.
+//
+// Bound by HBM: the logits are read once and the gradient written once, 8
+// bytes per logit. A cluster of CTAs shares a row and each thread keeps its
+// part, up to 32 logits, in registers between the two: 64 registers a thread,
+// so an SM holds 128 KB of rows, and with several clusters resident the reads
+// of some rows overlap the exponentials and writes of others. A row of more
+// than 8 x 16384 logits goes through the registers in tiles, and its gradient
+// pass reads it again (from L2). The CTAs' maxima and sums meet in
+// distributed shared memory. Warp 0 of each CTA works out the teacher's list
+// while the row is on its way; the listed classes of a CTA's part are written
+// once more at the end, with the teacher's and the label's terms.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -19,14 +27,16 @@
 #include <cfloat>
 #include <cmath>
 
+#include "pdl.cuh"
 #include "ttk_common.cuh"
 #include "ttk_internal.h"
 
 namespace ttk {
 namespace distill {
 
-constexpr int THREADS = 512;
-constexpr int WARPS = THREADS / 32;
+constexpr int MAX_THREADS = 512;
+constexpr int WORDS = 8;     // float4 words of a row per thread
+constexpr int MAX_CTAS = 8;  // of a cluster (the portable limit)
 constexpr int MAX_K = 1024;  // entries of one teacher list
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -60,188 +70,286 @@ __device__ __forceinline__ float exp_from(float x, float m, float c) {
     return exp2_approx((x - m) * c);
 }
 
-// Running (maximum, sum at temperature 1, sum at T) of part of a row.
+// (maximum, sum at temperature 1, sum at T) of part of a row.
 struct Stat {
     float m, s1, sT;
 };
 
-__device__ __forceinline__ void push(Stat& a, float x, float cT) {
-    if (x > a.m) {
-        if (a.m > -INFINITY) {
-            a.s1 *= exp_from(a.m, x, LOG2E);
-            a.sT *= exp_from(a.m, x, cT);
-        }
-        a.m = x;
-    }
-    // -inf adds nothing (and -inf - -inf would be NaN); NaN reaches the sums
-    if (!(x == -INFINITY)) {
-        a.s1 += exp_from(x, a.m, LOG2E);
-        a.sT += exp_from(x, a.m, cT);
-    }
-}
-
-__device__ __forceinline__ Stat merge(const Stat& a, const Stat& b, float cT) {
+// The statistics held by the lanes of a warp, as one, in every lane.
+__device__ __forceinline__ Stat warp_merge(const Stat& a, float cT) {
     Stat r;
-    r.m = fmaxf(a.m, b.m);
+    r.m = warp_max(a.m);
     const float z = r.m == -INFINITY ? 0.0f : r.m;
-    r.s1 = a.s1 * exp_from(a.m, z, LOG2E) + b.s1 * exp_from(b.m, z, LOG2E);
-    r.sT = a.sT * exp_from(a.m, z, cT) + b.sT * exp_from(b.m, z, cT);
+    r.s1 = warp_sum(a.s1 * exp_from(a.m, z, LOG2E));
+    r.sT = warp_sum(a.sT * exp_from(a.m, z, cT));
     return r;
 }
 
-__device__ float block_max(float v, float* red) {
-    v = warp_max(v);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0)
-        red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = red[threadIdx.x & (WARPS - 1)];
-    return warp_max(v);
+__device__ __forceinline__ Stat load_stat(const Stat* p, uint32_t rank) {
+    const uint32_t addr = smem_in_cta(p, rank);
+    Stat r;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(r.m) : "r"(addr) : "memory");
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(r.s1) : "r"(addr + 4) : "memory");
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(r.sT) : "r"(addr + 8) : "memory");
+    return r;
 }
 
-__device__ double block_sum(double v, double* red) {
-    v = warp_sum_d(v);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0)
-        red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    double s = 0.0;
-    for (int i = 0; i < WARPS; ++i)
-        s += red[i];
-    return s;
+__device__ __forceinline__ void store_cluster(double* p, uint32_t rank, double v) {
+    asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(smem_in_cta(p, rank)), "d"(v) : "memory");
 }
 
-__global__ void __launch_bounds__(THREADS) distill_row_kernel(const Args a) {
-    __shared__ Stat s_stat[WARPS];
-    __shared__ float s_red[WARPS];
-    __shared__ double s_redd[WARPS];
-    __shared__ int s_id[MAX_K + 1];
-    __shared__ float s_coef[MAX_K + 1];  // teacher's and label's gradient per entry
-    const int tid = threadIdx.x;
+__device__ __forceinline__ void cluster_arrive() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// TWO: both temperatures' sums are needed; otherwise T alone (T = 1, or no
+// labels). The row is cut into 16-byte words from the boundary at or before
+// its start: `off` floats of the first word belong to the row before.
+template <bool TWO>
+__global__ void __launch_bounds__(MAX_THREADS, 2) row_kernel(const Args a, const int ctas) {
+    extern __shared__ float dyn[];
+    __shared__ Stat s_warp[MAX_THREADS / 32];
+    __shared__ Stat s_cta;
+    __shared__ float s_flags[2];         // list has entries, label in range
+    __shared__ double s_kd[MAX_CTAS];    // in the cluster's first CTA
+    __shared__ double s_ce[MAX_CTAS];
+    const int C = static_cast<int>(a.C), K = static_cast<int>(a.K), pad = (K + 4) / 4 * 4;
+    int* const s_id = reinterpret_cast<int*>(dyn);  // [K + 1]: -1 where not in this CTA's part
+    float* const s_p = dyn + pad;                   // probability; gradient of the label
+    float* const s_a = dyn + 2 * pad;               // log p
+    float* const s_x = dyn + 3 * pad;               // the student's logit
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, T = blockDim.x;
+    const uint32_t rank = cluster_ctarank();
     const float cT = LOG2E / a.temperature, invT = 1.0f / a.temperature;
-    const int K = static_cast<int>(a.K);
-    for (int64_t row = blockIdx.x; row < a.N; row += gridDim.x) {
+    grid_wait();
+    for (int64_t row = blockIdx.x / ctas; row < a.N; row += gridDim.x / ctas) {
+        const float* const xr = a.logits + row * a.ld;
+        float* const dr = a.dlogits ? a.dlogits + row * a.ldd : nullptr;
         const float w = a.row_weight ? a.row_weight[row] : 1.0f;
-        float* dr = a.dlogits ? a.dlogits + row * a.ldd : nullptr;
-        // The teacher's list and the label. NaN counts as present: it has to
-        // reach the row's result.
-        __syncthreads();  // s_id, s_coef: the previous row is done with them
-        float zmax = -INFINITY;
-        for (int k = tid; k < K; k += THREADS) {
-            const int id = a.ids[row * a.K + k];
-            const bool ok = id >= 0 && id < a.C;
-            if (!ok && id != -1)
-                report(kErrBadIndex);
-            const float z = ok ? load_top(a.top, a.top_type, row * a.K + k) * invT : -INFINITY;
-            s_id[k] = ok ? id : -1;
-            s_coef[k] = z;
-            zmax = fmaxf(zmax, z != z ? INFINITY : z);
-        }
-        zmax = block_max(zmax, s_red);
-        const bool has = zmax > -INFINITY;
-        const int64_t t = a.targets ? a.targets[row] : -1;
-        const bool t_ok = t >= 0 && t < a.C;
-        if (tid == 0 && !t_ok && t != -1)
-            report(kErrBadIndex);
-        if (w == 0.0f || (!has && !t_ok)) {  // nothing to learn from: the row is not read
+        const int off = static_cast<int>((reinterpret_cast<uintptr_t>(xr) & 15) >> 2);
+        const int words = (off + C + 3) / 4, part = (words + ctas - 1) / ctas;
+        const int w0 = static_cast<int>(rank) * part, w1 = min(words, w0 + part);
+        // gradient words are aligned as the logits' are
+        const bool same = ((reinterpret_cast<uintptr_t>(xr) ^ reinterpret_cast<uintptr_t>(dr)) & 15) == 0;
+        auto store = [&](int wd, const float (&g)[4]) {
+            const int c = 4 * wd - off;
+            if (same && c >= 0 && c + 4 <= C) {
+                *reinterpret_cast<float4*>(dr + c) = make_float4(g[0], g[1], g[2], g[3]);
+            } else {
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (c + u >= 0 && c + u < C)
+                        dr[c + u] = g[u];
+            }
+        };
+        const float zeros[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (w == 0.0f) {  // masked row: its logits are not looked at
             if (dr)
-                for (int64_t c = tid; c < a.C; c += THREADS)
-                    dr[c] = 0.0f;
-            if (tid == 0)
+                for (int wd = w0 + tid; wd < w1; wd += T)
+                    store(wd, zeros);
+            if (rank == 0 && tid == 0)
                 a.terms[2 * row] = a.terms[2 * row + 1] = 0.0;
             continue;
         }
-        const float* xr = a.logits + row * a.ld;
-        Stat st{-INFINITY, 0.0f, 0.0f};
-        for (int64_t c = tid; c < a.C; c += THREADS)
-            push(st, xr[c], cT);
-        for (int o = 16; o > 0; o >>= 1) {
-            Stat b{__shfl_xor_sync(~0u, st.m, o), __shfl_xor_sync(~0u, st.s1, o),
-                   __shfl_xor_sync(~0u, st.sT, o)};
-            st = merge(st, b, cT);
-        }
-        __syncthreads();
-        if ((tid & 31) == 0)
-            s_stat[tid >> 5] = st;
-        __syncthreads();
-        st = s_stat[0];
-        for (int i = 1; i < WARPS; ++i)
-            st = merge(st, s_stat[i], cT);
-        const float m = st.m, log1 = logf(st.s1), logT = logf(st.sT);
-
-        // Teacher probabilities, KD, gradient coefficients.
-        double sz = 0.0;
-        if (has)
-            for (int k = tid; k < K; k += THREADS)
-                if (s_id[k] >= 0)
-                    sz += expf(s_coef[k] - zmax);
-        sz = block_sum(sz, s_redd);
-        const float logz = logf(static_cast<float>(sz)), invz = static_cast<float>(1.0 / sz);
-        const float gs = a.grad_scale * w;
-        const float gT = gs * a.alpha * a.temperature;
-        double kd = 0.0;
-        if (has)
-            for (int k = tid; k < K; k += THREADS) {
-                float p = 0.0f;
-                if (s_id[k] >= 0) {
-                    const float z = s_coef[k] - zmax;
-                    p = expf(z) * invz;
-                    if (p != 0.0f)
-                        kd += static_cast<double>(p * ((z - logz) - ((xr[s_id[k]] - m) * invT - logT)));
+        // The row's part, tile by tile; the last tile stays in x.
+        const int per = T * WORDS, tiles = (part + per - 1) / per;
+        float x[4 * WORDS];
+        auto load = [&](int tile) {
+#pragma unroll
+            for (int j = 0; j < WORDS; ++j) {
+                const int wd = w0 + tile * per + j * T + tid, c = 4 * wd - off;
+                float4 v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                if (wd < w1) {
+                    if (c >= 0 && c + 4 <= C) {
+                        v = *reinterpret_cast<const float4*>(xr + c);
+                    } else {
+                        if (c >= 0)
+                            v.x = xr[c];
+                        if (c + 1 >= 0 && c + 1 < C)
+                            v.y = xr[c + 1];
+                        if (c + 2 >= 0 && c + 2 < C)
+                            v.z = xr[c + 2];
+                        if (c + 3 < C)
+                            v.w = xr[c + 3];
+                    }
                 }
-                s_coef[k] = gT * p;
+                x[4 * j] = v.x, x[4 * j + 1] = v.y, x[4 * j + 2] = v.z, x[4 * j + 3] = v.w;
             }
-        else
-            for (int k = tid; k < K; k += THREADS)
-                s_coef[k] = 0.0f;
-        kd = block_sum(kd, s_redd);
-        const float g1 = t_ok ? gs * (1.0f - a.alpha) : 0.0f;
-        if (tid == 0) {
-            s_id[K] = t_ok ? static_cast<int>(t) : -1;
-            s_coef[K] = g1;
-            a.terms[2 * row] = w * kd;
-            a.terms[2 * row + 1] = t_ok ? static_cast<double>(w) * (log1 + (m - xr[t])) : 0.0;
-        }
-        if (!dr)
-            continue;
-        // Gradient without the listed terms; entries of the list are read
-        // before the row is overwritten (dlogits may be logits).
-        const float k1 = t_ok ? g1 / st.s1 : 0.0f, kT = has ? gT / st.sT : 0.0f;
-        auto base = [&](float x) {
-            return kT * exp_from(x, m, cT) + k1 * exp_from(x, m, LOG2E);
         };
-        __syncthreads();
-        constexpr int PER = (MAX_K + 1 + THREADS - 1) / THREADS;
-        float fix[PER];
-        bool write[PER];
+        load(0);
+        if (warp == 0) {
+            // The teacher's list. NaN counts as present: it has to reach the
+            // row's result.
+            float zmax = -INFINITY;
+            for (int k = lane; k < K; k += 32) {
+                const int id = a.ids[row * a.K + k];
+                const bool ok = id >= 0 && id < C;
+                if (!ok && id != -1 && rank == 0)
+                    report(kErrBadIndex);
+                const float z = ok ? load_top(a.top, a.top_type, row * a.K + k) * invT : -INFINITY;
+                const int wd = ok ? (id + off) >> 2 : -1;
+                const bool here = wd >= w0 && wd < w1;
+                s_id[k] = here ? id : -1;
+                s_a[k] = z;
+                s_x[k] = here ? xr[id] : 0.0f;
+                zmax = fmaxf(zmax, z != z ? INFINITY : z);
+            }
+            zmax = warp_max(zmax);
+            const bool has = zmax > -INFINITY;
+            float sz = 0.0f;
+            if (has)
+                for (int k = lane; k < K; k += 32)
+                    sz += expf(s_a[k] - zmax);
+            sz = warp_sum(sz);
+            const float logz = logf(sz), invz = 1.0f / sz;
+            for (int k = lane; k < K; k += 32) {
+                s_p[k] = has ? expf(s_a[k] - zmax) * invz : 0.0f;
+                s_a[k] = has ? (s_a[k] - zmax) - logz : 0.0f;
+            }
+            if (lane == 0) {
+                const int64_t t = a.targets ? a.targets[row] : -1;
+                const bool ok = t >= 0 && t < C;
+                if (!ok && t != -1 && rank == 0)
+                    report(kErrBadIndex);
+                const int wd = ok ? (static_cast<int>(t) + off) >> 2 : -1;
+                const bool here = wd >= w0 && wd < w1;
+                s_id[K] = here ? static_cast<int>(t) : -1;
+                s_x[K] = here ? xr[t] : 0.0f;
+                s_flags[0] = has ? 1.0f : 0.0f;
+                s_flags[1] = ok ? 1.0f : 0.0f;
+            }
+            __syncwarp();
+        }
+        // Statistics: the warp's maximum first, so that the sums need no
+        // rescaling but between tiles.
+        Stat st{-INFINITY, 0.0f, 0.0f};
+        for (int tile = 0;;) {
+            float m = x[0];
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int k = i * THREADS + tid;
-            fix[i] = 0.0f;
-            write[i] = false;
-            if (k <= K && s_id[k] >= 0) {
-                // the first entry of a class carries all of its entries, in list order
+            for (int i = 1; i + 1 < 4 * WORDS; i += 2)
+                m = max3(m, x[i], x[i + 1]);
+            m = warp_max(fmaxf(m, x[4 * WORDS - 1]));
+            m = fmaxf(st.m, m);
+            const float z = m == -INFINITY ? 0.0f : m;  // -inf - -inf would be NaN
+            if (tile) {
+                st.s1 *= exp_from(st.m, z, LOG2E);
+                st.sT *= exp_from(st.m, z, cT);
+            }
+#pragma unroll
+            for (int i = 0; i < 4 * WORDS; ++i) {
+                if constexpr (TWO)
+                    st.s1 += exp_from(x[i], z, LOG2E);
+                st.sT += exp_from(x[i], z, cT);
+            }
+            st.m = m;
+            if (++tile >= tiles)
+                break;
+            load(tile);
+        }
+        if constexpr (!TWO)
+            st.s1 = st.sT;
+        st.s1 = warp_sum(st.s1);
+        st.sT = warp_sum(st.sT);
+        if (lane == 0)
+            s_warp[warp] = st;
+        __syncthreads();
+        const Stat none{-INFINITY, 0.0f, 0.0f};
+        st = warp_merge(lane < (T >> 5) ? s_warp[lane] : none, cT);
+        if (ctas > 1) {
+            if (tid == 0)
+                s_cta = st;
+            cluster_arrive();
+            cluster_wait();
+            st = warp_merge(lane < ctas ? load_stat(&s_cta, lane) : none, cT);
+        }
+        const bool has = s_flags[0] != 0.0f, t_ok = s_flags[1] != 0.0f;
+        const float m = st.m, logT = logf(st.sT);
+        const float gs = a.grad_scale * w;
+        const float gT = has ? gs * a.alpha * a.temperature : 0.0f;
+        const float g1 = t_ok ? gs * (1.0f - a.alpha) : 0.0f;
+        if (warp == 0) {  // this CTA's share of the loss, to the cluster's first CTA
+            double kd = 0.0;
+            for (int k = lane; k < K; k += 32)
+                if (s_id[k] >= 0 && s_p[k] != 0.0f)
+                    kd += static_cast<double>(s_p[k] * (s_a[k] - ((s_x[k] - m) * invT - logT)));
+            kd = warp_sum_d(kd);
+            if (lane == 0) {
+                const double ce = s_id[K] >= 0 ? static_cast<double>(logf(st.s1) + (m - s_x[K])) : 0.0;
+                if (ctas > 1) {
+                    store_cluster(s_kd + rank, 0, kd);
+                    store_cluster(s_ce + rank, 0, ce);
+                } else {
+                    a.terms[2 * row] = w * kd;
+                    a.terms[2 * row + 1] = w * ce;
+                }
+            }
+            __syncwarp();
+        }
+        if (ctas > 1)
+            cluster_arrive();
+        const float k1 = t_ok ? g1 / st.s1 : 0.0f, kT = has ? gT / st.sT : 0.0f;
+        const bool use1 = TWO && k1 != 0.0f, useT = !TWO || kT != 0.0f;
+        const float kk = TWO ? kT : (t_ok ? k1 : 0.0f) + kT;  // one temperature: one term
+        auto base = [&](float v) {
+            float g = useT ? kk * exp_from(v, m, cT) : 0.0f;
+            if (use1)
+                g += k1 * exp_from(v, m, LOG2E);
+            return g;
+        };
+        if (dr) {
+            for (int tile = tiles - 1;;) {
+#pragma unroll
+                for (int j = 0; j < WORDS; ++j) {
+                    const int wd = w0 + tile * per + j * T + tid;
+                    float g[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    if (has || t_ok)
+#pragma unroll
+                        for (int u = 0; u < 4; ++u)
+                            g[u] = base(x[4 * j + u]);
+                    if (wd < w1)
+                        store(wd, g);
+                }
+                if (--tile < 0)
+                    break;
+                load(tile);
+            }
+            __syncthreads();
+            // The listed classes: the first entry of a class carries all of
+            // its entries, in list order, then the label.
+            for (int k = tid; k <= K; k += T) {
+                const int id = s_id[k];
+                if (id < 0)
+                    continue;
                 bool first = true;
-                for (int j = 0; j < k; ++j)
-                    first = first && s_id[j] != s_id[k];
                 float sum = 0.0f;
+                for (int j = 0; j < K; ++j)
+                    if (s_id[j] == id) {
+                        first = first && j >= k;
+                        sum += s_p[j];
+                    }
                 if (first)
-                    for (int j = k; j <= K; ++j)
-                        sum += s_id[j] == s_id[k] ? s_coef[j] : 0.0f;
-                if (first)
-                    fix[i] = base(xr[s_id[k]]) - sum;
-                write[i] = first;
+                    dr[id] = base(s_x[k]) - (gT * sum + (s_id[K] == id ? g1 : 0.0f));
             }
         }
-        __syncthreads();
-        for (int64_t c = tid; c < a.C; c += THREADS)
-            dr[c] = base(xr[c]);
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int k = i * THREADS + tid;
-            if (write[i])
-                dr[s_id[k]] = fix[i];
+        if (ctas > 1) {
+            cluster_wait();
+            if (rank == 0 && tid == 0) {
+                double kd = 0.0, ce = 0.0;
+                for (int i = 0; i < ctas; ++i)
+                    kd += s_kd[i], ce += s_ce[i];
+                a.terms[2 * row] = w * kd;
+                a.terms[2 * row + 1] = w * ce;
+            }
+        }
+        if (row + gridDim.x / ctas < a.N) {  // shared memory is free for the next row
+            __syncthreads();
+            if (ctas > 1) {
+                cluster_arrive();
+                cluster_wait();
+            }
         }
     }
 }
@@ -254,9 +362,12 @@ __global__ void __launch_bounds__(1024) distill_sum_kernel(const double* __restr
                                                            float* __restrict__ loss) {
     __shared__ double red[2][32];
     double kd = 0.0, ce = 0.0;
+    grid_wait();
+#pragma unroll 4
     for (int64_t i = threadIdx.x; i < N; i += blockDim.x) {
-        kd += terms[2 * i];
-        ce += terms[2 * i + 1];
+        const double2 t = reinterpret_cast<const double2*>(terms)[i];
+        kd += t.x;
+        ce += t.y;
     }
     kd = warp_sum_d(kd);
     ce = warp_sum_d(ce);
@@ -279,6 +390,37 @@ __global__ void __launch_bounds__(1024) distill_sum_kernel(const double* __restr
     }
 }
 
+// As few CTAs to a row as hold it in registers; more, of at least 2048 logits
+// each, while the rows do not fill the machine.
+template <bool TWO>
+int launch_rows(const Args& a, cudaStream_t st) {
+    const int64_t words = (a.C + 6) / 4, cap = static_cast<int64_t>(MAX_THREADS) * WORDS;
+    int ctas = static_cast<int>(std::min<int64_t>(MAX_CTAS, (words + cap - 1) / cap));
+    while (ctas * 2 <= MAX_CTAS && a.N * ctas * 2 <= 148 * 8 && words / (ctas * 2) >= 512)
+        ctas *= 2;
+    const int64_t part = (words + ctas - 1) / ctas;
+    const int threads = static_cast<int>(
+        std::min<int64_t>(MAX_THREADS, ((part + WORDS - 1) / WORDS + 31) / 32 * 32));
+    const int64_t rows = std::min<int64_t>(a.N, (1 << 30) / ctas);
+    const size_t smem = static_cast<size_t>((a.K + 4) / 4 * 4) * 4 * sizeof(float);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(rows * ctas));
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(ctas);
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, row_kernel<TWO>, a, ctas);
+    const int rc = check_launch("distill_loss");
+    return rc ? rc : check_cuda(e, "distill_loss");
+}
+
 }  // namespace distill
 }  // namespace ttk
 
@@ -296,7 +438,7 @@ int ttk_distill_loss(const float* logits, int64_t ld, const int32_t* teacher_ids
                      const int64_t* targets, const float* row_weight, int64_t N, int64_t C,
                      float alpha, float temperature, float grad_scale, float* loss, float* dlogits,
                      int64_t ldd, void* workspace, size_t workspace_bytes, void* stream) {
-    if (N < 0 || C <= 0 || C > INT32_MAX || K < 0 || !loss || (N && !logits))
+    if (N < 0 || C <= 0 || C > (1 << 30) || K < 0 || !loss || (N && !logits))
         return set_error(TTK_ERR_ARG, "distill_loss: bad arguments");
     if (ld < C || (dlogits && ldd < C))
         return set_error(TTK_ERR_ARG, "distill_loss: a row stride is shorter than the row");
@@ -314,20 +456,20 @@ int ttk_distill_loss(const float* logits, int64_t ld, const int32_t* teacher_ids
         return set_error(TTK_ERR_ARG, "distill_loss: in place needs equal row strides");
     if (N && (!workspace || workspace_bytes < ttk_distill_loss_workspace_size(N)))
         return set_error(TTK_ERR_ARG, "distill_loss: workspace too small");
-    if (reinterpret_cast<uintptr_t>(workspace) & 7)
-        return set_error(TTK_ERR_ARG, "distill_loss: workspace must be 8-byte aligned");
+    if (reinterpret_cast<uintptr_t>(workspace) & 15)
+        return set_error(TTK_ERR_ARG, "distill_loss: workspace must be 16-byte aligned");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     double* terms = static_cast<double*>(workspace);
     if (N) {
         const Args a{logits, ld, teacher_ids, teacher_logits, teacher_type, K, targets, row_weight,
                      N, C, alpha, temperature, grad_scale, terms, dlogits, ldd};
-        distill_row_kernel<<<grid_for(N, 1, 148 * 4), THREADS, 0, st>>>(a);
-        const int rc = check_launch("distill_row_kernel");
+        const bool two = temperature != 1.0f && targets;
+        const int rc = two ? launch_rows<true>(a, st) : launch_rows<false>(a, st);
         if (rc)
             return rc;
     }
-    distill_sum_kernel<<<1, 1024, 0, st>>>(terms, N, alpha, temperature, grad_scale, loss);
-    return check_launch("distill_sum_kernel");
+    return launch_pdl("distill_loss sum", distill_sum_kernel, dim3(1), 1024, 0, st,
+                      static_cast<const double*>(terms), N, alpha, temperature, grad_scale, loss);
 }
 
 }  // extern "C"

@@ -9,6 +9,7 @@
 
 #include <algorithm>
 
+#include "pdl.cuh"
 #include "ttk_common.cuh"
 #include "ttk_internal.h"
 
@@ -51,6 +52,7 @@ __global__ void __launch_bounds__(256) lookup_kernel(const float* __restrict__ W
     const int lane = threadIdx.x & 31;
     const int64_t item = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
     const int64_t i = item / pieces, words = D / VEC, w0 = (item - i * pieces) * 128 + lane;
+    grid_wait();
     if (i >= N)
         return;
     const int64_t t = idx[i];
@@ -70,20 +72,29 @@ __global__ void __launch_bounds__(256) lookup_kernel(const float* __restrict__ W
 }
 
 // ---------------------------------------------------------------- sorting --
-// Stable radix sort of (token, position) by one cluster of 8 blocks, 8 bits
-// a pass. Each warp owns a contiguous run of the keys: it counts its digits,
-// the counts are scanned over the warps of the block and over the blocks
-// (through distributed shared memory), and the warp then writes its keys in
-// order. Tokens outside [0, V) become V and end up last.
-// The sort occupies 8 SMs; when dW is written (not added to), the launch's
-// other clusters meanwhile zero the rows of tokens that do not occur. Each of
-// their blocks owns a range of rows and marks the tokens of that range in a
-// bitmap of its own by reading all the ids (from L2), so it waits for nobody.
+// (token, position) pairs in ascending order, tokens outside [0, V) as V, so
+// last. Two ways:
+//   rank_kernel, up to 8192 positions: every pair is packed into 32 bits, and
+//     a pair's place is the number of smaller ones, counted by one warp over
+//     all of them in shared memory. No step waits for another.
+//   radix_kernel: a stable radix sort by one cluster of 8 blocks, 8 bits a
+//     pass. Each warp owns a contiguous run of the pairs: it counts its digits,
+//     the counts are scanned over the warps of the block and over the blocks
+//     (through distributed shared memory), and the warp writes its pairs in
+//     order.
+// Neither needs the whole machine; when dW is written (not added to), the
+// launch's other blocks meanwhile zero the rows of tokens that do not occur.
+// Each owns a range of rows and marks the range's tokens in a bitmap of its
+// own by reading all the ids (from L2), so it waits for nobody.
 constexpr int SORT_CTAS = 8;
 constexpr int SORT_THREADS = 1024;
 constexpr int SORT_WARPS = SORT_THREADS / 32;
 constexpr int RADIX = 256;
 constexpr int64_t ROWS_A_ROUND = RADIX * SORT_WARPS * 32;  // rows one bitmap covers
+constexpr int RANK_BITS = 13;
+constexpr int64_t RANK_MAX = 1 << RANK_BITS;
+constexpr int RANK_THREADS = 256;
+constexpr int RANK_KEYS = 4;  // places a warp counts at once
 
 // Rows [v0, v1) of dW that no id names are set to zero. VEC as above.
 template <int VEC>
@@ -94,24 +105,78 @@ __device__ void zero_absent(const int64_t* __restrict__ idx, int64_t N, int64_t 
     for (int64_t a = v0; a < v1; a += ROWS_A_ROUND) {
         const int64_t e = min(v1, a + ROWS_A_ROUND);
         __syncthreads();
-        for (int64_t i = threadIdx.x; i < (e - a + 31) / 32; i += SORT_THREADS)
+        for (int64_t i = threadIdx.x; i < (e - a + 31) / 32; i += blockDim.x)
             bits[i] = 0;
         __syncthreads();
 #pragma unroll 4
-        for (int64_t i = threadIdx.x; i < N; i += SORT_THREADS) {
+        for (int64_t i = threadIdx.x; i < N; i += blockDim.x) {
             const int64_t t = idx[i];
             if (t >= a && t < e)
                 atomicOr(bits + ((t - a) >> 5), 1u << ((t - a) & 31));
         }
         __syncthreads();
         const int lane = threadIdx.x & 31;
-        for (int64_t v = a + (threadIdx.x >> 5); v < e; v += SORT_WARPS)
+        for (int64_t v = a + (threadIdx.x >> 5); v < e; v += blockDim.x >> 5)
             if (!((bits[(v - a) >> 5] >> ((v - a) & 31)) & 1u)) {
                 T* row = reinterpret_cast<T*>(dW + v * D);
 #pragma unroll 4
                 for (int64_t c = lane; c < words; c += 32)
                     row[c] = zero<T>();
             }
+    }
+}
+
+template <int VEC>
+__global__ void __launch_bounds__(RANK_THREADS)
+    rank_kernel(const int64_t* __restrict__ idx, int N, int64_t V, int sorters,
+                uint64_t* __restrict__ keys, uint32_t* __restrict__ count, float* __restrict__ dW,
+                int64_t D) {
+    __shared__ __align__(16) uint32_t pairs[RANK_MAX];
+    static_assert(RANK_MAX * 32 >= ROWS_A_ROUND, "the pairs' memory holds a bitmap");
+    grid_wait();
+    if (static_cast<int>(blockIdx.x) >= sorters) {
+        const int64_t nz = gridDim.x - sorters, z = blockIdx.x - sorters;
+        zero_absent<VEC>(idx, N, V * z / nz, V * (z + 1) / nz, dW, D, pairs);
+        return;
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0)
+        *count = 0;
+    for (int i = threadIdx.x; i < (N + 3) / 4 * 4; i += RANK_THREADS) {
+        uint32_t p = ~0u;  // no pair: greater than all of them
+        if (i < N) {
+            const int64_t t = idx[i];
+            const bool live = t >= 0 && t < V;
+            if (!live && t != -1 && blockIdx.x == 0)
+                report(kErrBadIndex);
+            p = static_cast<uint32_t>(live ? t : V) << RANK_BITS | static_cast<uint32_t>(i);
+        }
+        pairs[i] = p;
+    }
+    __syncthreads();
+    const int lane = threadIdx.x & 31;
+    for (int i0 = (blockIdx.x * (RANK_THREADS / 32) + (threadIdx.x >> 5)) * RANK_KEYS; i0 < N;
+         i0 += sorters * (RANK_THREADS / 32) * RANK_KEYS) {
+        uint32_t mine[RANK_KEYS];
+        int below[RANK_KEYS];
+#pragma unroll
+        for (int k = 0; k < RANK_KEYS; ++k) {
+            mine[k] = pairs[min(i0 + k, N - 1)];
+            below[k] = 0;
+        }
+#pragma unroll 4
+        for (int j = lane; j < (N + 3) / 4; j += 32) {
+            const uint4 v = reinterpret_cast<const uint4*>(pairs)[j];
+#pragma unroll
+            for (int k = 0; k < RANK_KEYS; ++k)
+                below[k] += (v.x < mine[k]) + (v.y < mine[k]) + (v.z < mine[k]) + (v.w < mine[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < RANK_KEYS; ++k) {
+            const int place = __reduce_add_sync(~0u, below[k]);
+            if (lane == k && i0 + k < N)
+                keys[place] = static_cast<uint64_t>(mine[k] >> RANK_BITS) << 32 |
+                              (mine[k] & (RANK_MAX - 1));
+        }
     }
 }
 
@@ -123,19 +188,22 @@ __device__ __forceinline__ uint32_t ld_cluster(const uint32_t* p, uint32_t rank)
 
 template <int VEC>
 __global__ void __cluster_dims__(SORT_CTAS, 1, 1) __launch_bounds__(SORT_THREADS)
-    sort_kernel(const int64_t* __restrict__ idx, int64_t N, int64_t V, int passes,
-                uint64_t* __restrict__ bufa, uint64_t* __restrict__ bufb, float* __restrict__ dW,
-                int64_t D) {
+    radix_kernel(const int64_t* __restrict__ idx, int64_t N, int64_t V, int passes,
+                 uint64_t* __restrict__ bufa, uint64_t* __restrict__ bufb,
+                 uint32_t* __restrict__ count, float* __restrict__ dW, int64_t D) {
     __shared__ uint32_t hist[SORT_WARPS][RADIX];
     __shared__ uint32_t total[RADIX];
     __shared__ uint32_t wsum[8];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    grid_wait();
     if (blockIdx.x >= SORT_CTAS) {  // whole clusters
         const int64_t nz = gridDim.x - SORT_CTAS, z = blockIdx.x - SORT_CTAS;
         zero_absent<VEC>(idx, N, V * z / nz, V * (z + 1) / nz, dW, D, &hist[0][0]);
         return;
     }
     const uint32_t rank = cluster_ctarank();
+    if (rank == 0 && tid == 0)
+        *count = 0;
     const int64_t nwarps = SORT_CTAS * SORT_WARPS;
     const int64_t per = ((N + nwarps - 1) / nwarps + 31) / 32 * 32;
     const int64_t lo = (static_cast<int64_t>(rank) * SORT_WARPS + warp) * per;
@@ -227,9 +295,10 @@ __global__ void __cluster_dims__(SORT_CTAS, 1, 1) __launch_bounds__(SORT_THREADS
 // thread one word of the row, and writes dW where a token's run ends. A run
 // that crosses chunks leaves partial sums in part[chunk][0] (the chunk's
 // first run, when it began earlier) and part[chunk][1] (its last run, when it
-// began here and goes on); join_kernel adds those. So frequent tokens are
-// spread over many blocks, and the order of every sum depends on N, D and the
-// ids alone.
+// began here and goes on), and the chunk where it began goes on the list that
+// join_kernel adds up. So frequent tokens are spread over many blocks, and the
+// order of every sum depends on N, D and the ids alone (that of the list does
+// not matter).
 constexpr int MAX_L = 64;
 constexpr int DEPTH = 8;  // rows in flight per thread
 
@@ -239,12 +308,14 @@ template <int VEC>
 __global__ void __launch_bounds__(256)
     chunk_kernel(const uint64_t* __restrict__ keys, int64_t N, int L, const float* __restrict__ dout,
                  float* __restrict__ dW, int accumulate, int64_t D, int64_t V, float scale,
-                 float* __restrict__ part) {
+                 float* __restrict__ part, uint32_t* __restrict__ count,
+                 uint32_t* __restrict__ list) {
     using T = typename Vec<VEC>::T;
     __shared__ uint64_t s_key[MAX_L + 2];  // the chunk's keys, its neighbours on both sides
     const int64_t first = static_cast<int64_t>(blockIdx.x) * L;
     const int n = static_cast<int>(min(static_cast<int64_t>(L), N - first));
     const uint64_t none = ~0ull;
+    grid_wait();
     for (int i = threadIdx.x; i < n + 2; i += blockDim.x) {
         const int64_t p = first + i - 1;
         s_key[i] = p >= 0 && p < N ? keys[p] : none;
@@ -281,6 +352,8 @@ __global__ void __launch_bounds__(256)
             const bool earlier = start == 0 && key_token(key[-1]) == t;
             if (earlier || more) {
                 slots[earlier ? 0 : words] = acc;
+                if (!earlier && c == 0)
+                    list[atomicAdd(count, 1u)] = blockIdx.x;
             } else {
                 T* d = reinterpret_cast<T*>(dW) + static_cast<int64_t>(t) * words + c;
                 const T r = times(acc, scale);
@@ -292,43 +365,52 @@ __global__ void __launch_bounds__(256)
     }
 }
 
-// One block per chunk and 32 words of the row: where a run begins in this
-// chunk and goes on, its partial sums, eight interleaved sequences of chunks
-// added in order.
+// Runs that cross chunks: a block takes one listed chunk and 32 words of the
+// row at a time, and adds the partial sums in eight interleaved sequences of
+// chunks, then those in order.
 constexpr int JOIN_WAYS = 8;
+constexpr int JOIN_THREADS = 32 * JOIN_WAYS;
 template <int VEC>
-__global__ void __launch_bounds__(32 * JOIN_WAYS)
+__global__ void __launch_bounds__(JOIN_THREADS)
     join_kernel(const uint64_t* __restrict__ keys, int64_t N, int L, float* __restrict__ dW,
-                int accumulate, int64_t D, int64_t V, float scale, const float* __restrict__ part) {
+                int accumulate, int64_t D, float scale, const float* __restrict__ part,
+                const uint32_t* __restrict__ count, const uint32_t* __restrict__ list) {
     using T = typename Vec<VEC>::T;
     __shared__ T s_part[JOIN_WAYS][32];
     const int lane = threadIdx.x & 31, way = threadIdx.x >> 5;
-    const int64_t chunk = blockIdx.x, last = (chunk + 1) * L - 1;
-    if (last + 1 >= N)
-        return;
-    const uint32_t t = key_token(keys[last]);
-    if (t >= V || key_token(keys[last + 1]) != t ||
-        (key_token(keys[chunk * L]) == t && chunk && key_token(keys[chunk * L - 1]) == t))
-        return;
-    const int64_t words = D / VEC, c = static_cast<int64_t>(blockIdx.y) * 32 + lane;
-    const T* p = reinterpret_cast<const T*>(part) + c;
-    T acc = zero<T>();
-    if (c < words) {
-        if (way == 0)
-            acc = p[(2 * chunk + 1) * words];
-        // chunk k's first run is this token's while position k L is
-#pragma unroll 4
-        for (int64_t k = chunk + 1 + way; k * L < N && key_token(keys[k * L]) == t; k += JOIN_WAYS)
-            acc = plus(acc, p[2 * k * words]);
-    }
-    s_part[way][lane] = acc;
-    __syncthreads();
-    if (way == 0 && c < words) {
-        for (int i = 1; i < JOIN_WAYS; ++i)
-            acc = plus(acc, s_part[i][lane]);
-        T* d = reinterpret_cast<T*>(dW) + static_cast<int64_t>(t) * words + c;
-        const T r = times(acc, scale);
-        *d = accumulate ? plus(*d, r) : r;
+    const int64_t words = D / VEC, tiles = (words + 31) / 32;
+    grid_wait();
+    const int64_t items = static_cast<int64_t>(*count) * tiles;
+    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const int64_t chunk = list[item / tiles], c = item % tiles * 32 + lane;
+        const uint32_t t = key_token(keys[(chunk + 1) * L - 1]);
+        // chunks whose first run is this token's
+        int64_t more = 0;
+        int found;
+        do {
+            const int64_t p = (chunk + 1 + more + threadIdx.x) * L;
+            found = __syncthreads_count(p < N && key_token(keys[p]) == t);
+            more += found;
+        } while (found == JOIN_THREADS);
+        const T* p = reinterpret_cast<const T*>(part) + c;
+        T acc = zero<T>();
+        if (c < words) {
+            if (way == 0)
+                acc = p[(2 * chunk + 1) * words];
+#pragma unroll 8
+            for (int64_t k = chunk + 1 + way; k <= chunk + more; k += JOIN_WAYS)
+                acc = plus(acc, p[2 * k * words]);
+        }
+        s_part[way][lane] = acc;
+        __syncthreads();
+        if (way == 0 && c < words) {
+#pragma unroll
+            for (int i = 1; i < JOIN_WAYS; ++i)
+                acc = plus(acc, s_part[i][lane]);
+            T* d = reinterpret_cast<T*>(dW) + static_cast<int64_t>(t) * words + c;
+            const T r = times(acc, scale);
+            *d = accumulate ? plus(*d, r) : r;
+        }
     }
 }
 
@@ -358,33 +440,56 @@ Plan plan(int64_t N, int64_t D, bool aligned) {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+// Workspace: two key buffers, the list's count, the list, the partial rows.
+size_t workspace_bytes(const Plan& p, int64_t D) {
+    return 2 * p.keys + 16 + align16(static_cast<size_t>(p.chunks) * 4) +
+           static_cast<size_t>(p.chunks) * 2 * D * sizeof(float);
+}
+
 template <int VEC>
 int backward(const float* dout, const int64_t* idx, float* dW, int accumulate, int64_t N, int64_t D,
              int64_t V, float scale, char* ws, const Plan& p, cudaStream_t st) {
     uint64_t* bufa = reinterpret_cast<uint64_t*>(ws);
     uint64_t* bufb = reinterpret_cast<uint64_t*>(ws + p.keys);
-    float* part = reinterpret_cast<float*>(ws + 2 * p.keys);
-    int passes = 1;
-    while (passes < 4 && (V >> (8 * passes)))
-        ++passes;
-    // blocks that zero: at least 64 KB each, all clusters resident at once
-    const int64_t zero_ctas =
-        accumulate ? 0 : std::min<int64_t>(16, (V * D / (16384 * SORT_CTAS)) + 1) * SORT_CTAS;
-    sort_kernel<VEC><<<static_cast<int>(SORT_CTAS + zero_ctas), SORT_THREADS, 0, st>>>(
-        idx, N, V, passes, bufa, bufb, dW, D);
-    int rc = check_launch("embedding_scaled_bwd sort");
-    if (rc)
-        return rc;
-    const uint64_t* keys = (passes & 1) ? bufa : bufb;
-    chunk_kernel<VEC><<<dim3(static_cast<unsigned>(p.chunks), static_cast<unsigned>(p.tiles)),
-                        p.threads, 0, st>>>(keys, N, p.L, dout, dW, accumulate, D, V, scale, part);
-    rc = check_launch("embedding_scaled_bwd sums");
-    if (rc)
-        return rc;
-    join_kernel<VEC><<<dim3(static_cast<unsigned>(p.chunks),
-                            static_cast<unsigned>((p.words + 31) / 32)),
-                       32 * JOIN_WAYS, 0, st>>>(keys, N, p.L, dW, accumulate, D, V, scale, part);
-    return check_launch("embedding_scaled_bwd join");
+    uint32_t* count = reinterpret_cast<uint32_t*>(ws + 2 * p.keys);
+    uint32_t* list = count + 4;
+    float* part = reinterpret_cast<float*>(ws + 2 * p.keys + 16 +
+                                           align16(static_cast<size_t>(p.chunks) * 4));
+    const uint64_t* keys = bufa;
+    int rc;
+    if (N <= RANK_MAX && V < (1ll << (32 - RANK_BITS)) - 1) {
+        const int per = RANK_THREADS / 32 * RANK_KEYS;
+        const int sorters = static_cast<int>(std::min<int64_t>((N + per - 1) / per, 128));
+        // 32 KB of rows a zeroing block, several blocks an SM
+        const int64_t zeros = accumulate ? 0 : std::min<int64_t>(148 * 5, V * D / 8192 + 1);
+        rc = launch_pdl("embedding_scaled_bwd rank", rank_kernel<VEC>,
+                        dim3(static_cast<unsigned>(sorters + zeros)), RANK_THREADS, 0, st, idx,
+                        static_cast<int>(N), V, sorters, bufa, count, dW, D);
+    } else {
+        int passes = 1;
+        while (passes < 4 && (V >> (8 * passes)))
+            ++passes;
+        // 64 KB of rows a zeroing block, all clusters resident at once
+        const int64_t zeros =
+            accumulate ? 0 : std::min<int64_t>(15, V * D / (16384 * SORT_CTAS) + 1) * SORT_CTAS;
+        rc = launch_pdl("embedding_scaled_bwd sort", radix_kernel<VEC>,
+                        dim3(static_cast<unsigned>(SORT_CTAS + zeros)), SORT_THREADS, 0, st, idx, N,
+                        V, passes, bufa, bufb, count, dW, D);
+        keys = (passes & 1) ? bufa : bufb;
+    }
+    if (!rc)
+        rc = launch_pdl("embedding_scaled_bwd sums", chunk_kernel<VEC>,
+                        dim3(static_cast<unsigned>(p.chunks), static_cast<unsigned>(p.tiles)),
+                        p.threads, 0, st, keys, N, p.L, dout, dW, accumulate, D, V, scale, part,
+                        count, list);
+    const int64_t items = p.chunks * ((p.words + 31) / 32);  // at most
+    if (!rc)
+        rc = launch_pdl("embedding_scaled_bwd join", join_kernel<VEC>,
+                        dim3(static_cast<unsigned>(std::min<int64_t>(items, 148 * 8))), JOIN_THREADS,
+                        0, st, keys, N, p.L, dW, accumulate, D, scale,
+                        static_cast<const float*>(part), static_cast<const uint32_t*>(count),
+                        static_cast<const uint32_t*>(list));
+    return rc;
 }
 
 }  // namespace embs
@@ -406,11 +511,9 @@ int ttk_embedding_scaled_fwd(const float* W, const int64_t* idx, float* out, int
     const int64_t pieces = ((vec ? D / 4 : D) + 127) / 128, blocks = (N * pieces + 7) / 8;
     if (blocks > INT32_MAX)
         return set_error(TTK_ERR_ARG, "embedding_scaled_fwd: N * D too large");
-    if (vec)
-        lookup_kernel<4><<<static_cast<int>(blocks), 256, 0, st>>>(W, idx, out, N, D, V, scale, pieces);
-    else
-        lookup_kernel<1><<<static_cast<int>(blocks), 256, 0, st>>>(W, idx, out, N, D, V, scale, pieces);
-    return check_launch("embedding_scaled_fwd");
+    return launch_pdl("embedding_scaled_fwd", vec ? lookup_kernel<4> : lookup_kernel<1>,
+                      dim3(static_cast<unsigned>(blocks)), 256, 0, st, W, idx, out, N, D, V, scale,
+                      pieces);
 }
 
 size_t ttk_embedding_scaled_bwd_workspace_size(int64_t N, int64_t D, int64_t V) {
@@ -418,7 +521,7 @@ size_t ttk_embedding_scaled_bwd_workspace_size(int64_t N, int64_t D, int64_t V) 
         return 16;
     // the scalar form's plan can have shorter chunks than the vector form's
     const Plan p = plan(N, D, true), q = plan(N, D, false);
-    return 2 * p.keys + static_cast<size_t>(std::max(p.chunks, q.chunks)) * 2 * D * sizeof(float);
+    return std::max(workspace_bytes(p, D), workspace_bytes(q, D));
 }
 
 int ttk_embedding_scaled_bwd(const float* dout, const int64_t* idx, float* dW, int accumulate,
@@ -438,7 +541,7 @@ int ttk_embedding_scaled_bwd(const float* dout, const int64_t* idx, float* dW, i
         return set_error(TTK_ERR_ARG,
                          "embedding_scaled_bwd: workspace too small or not 16-byte aligned");
     const Plan p = plan(N, D, aligned16(dout) && aligned16(dW));
-    if (p.tiles > 65535 || (p.words + 31) / 32 > 65535)
+    if (p.tiles > 65535)
         return set_error(TTK_ERR_ARG, "embedding_scaled_bwd: D too large");
     char* ws = static_cast<char*>(workspace);
     return p.vec == 4

@@ -15,7 +15,9 @@ from ._ttk import call
 
 
 def _s():
-    return torch.cuda.current_stream().cuda_stream
+    """The current stream's handle (torch.cuda.current_stream().cuda_stream, without the
+    Stream object: 0.2 instead of 3.2 us)."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _p(t):
@@ -25,7 +27,7 @@ def _p(t):
 def _chk(t, name, dtype=torch.float32, shape=None):
     if not (t.is_cuda and t.dtype == dtype and t.is_contiguous()):
         raise ValueError(f"{name}: expected a contiguous {str(dtype).split('.')[-1]} CUDA tensor")
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if shape is not None and t.shape != shape:
         raise ValueError(f"{name}: expected shape {list(shape)}, got {list(t.shape)}")
 
 
