@@ -287,3 +287,36 @@ def test_no_rows(cuda):
     ce = -l1.gather(1, t[:, None]).mean()
     assert abs(float(out[0][0]) - float(ce)) <= 60 * U * (float(ce) + 1)
     assert status() == 0
+
+
+@pytest.mark.parametrize("C", [40, 5000, 32000, 40000])
+def test_rows_at_the_lowest_value(cuda, C):
+    """Rows whose logits are all the type's lowest value are uniform, as softmax
+    has them; a part of a row at that value next to ordinary logits has
+    probability 0."""
+    from tinytrain_b200 import kernels as KN
+    low = torch.finfo(torch.float32).min
+    x = torch.full((3, C), low, device=cuda)
+    x[1, C - 3:] = torch.tensor([1.0, 2.0, 3.0], device=cuda)
+    x[2, :] = -math.inf
+    x[2, C // 2] = low
+    ids = torch.full((3, 1), C - 1, dtype=torch.int32, device=cuda)
+    ids[2] = C // 2
+    t = ids[:, 0].long()
+    for T in (1.0, 2.0):
+        loss, d = KN.distill_loss(x, ids, torch.zeros(3, 1, device=cuda), t, alpha=0.5,
+                                  temperature=T, grad_scale=1.0)
+        q = torch.zeros(2, 3, C, dtype=torch.float64, device=cuda)  # at T, at 1
+        for i, k in enumerate((1 / T, 1.0)):
+            q[i, 0] = 1.0 / C
+            q[i, 1, C - 3:] = torch.softmax(k * torch.tensor([1.0, 2.0, 3.0], dtype=torch.float64), 0)
+            q[i, 2, C // 2] = 1.0
+        hit = torch.zeros(3, C, dtype=torch.float64, device=cuda).scatter_(1, t[:, None], 1.0)
+        want = 0.5 * T * (q[0] - hit) + 0.5 * (q[1] - hit)
+        mag = 0.5 * T * (q[0] + hit) + 0.5 * (q[1] + hit)
+        c = 60 + C / 256
+        assert ((d.double() - want).abs() <= c * U * mag).all()
+        kd, ce = (-(torch.log(v[torch.arange(3, device=cuda), t])).sum() for v in q)
+        ref = torch.stack([0.5 * T * T * kd + 0.5 * ce, kd, ce])
+        assert ((loss.double() - ref).abs() <= c * U * (ref + 3)).all()
+    assert status() == 0
