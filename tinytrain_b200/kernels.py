@@ -7,6 +7,7 @@ single kernels; the training path itself runs in the C++ tt:: library.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
 
@@ -29,6 +30,23 @@ def _chk(t, name, dtype=torch.float32, shape=None):
         raise ValueError(f"{name}: expected a contiguous {str(dtype).split('.')[-1]} CUDA tensor")
     if shape is not None and t.shape != shape:
         raise ValueError(f"{name}: expected shape {list(shape)}, got {list(t.shape)}")
+
+
+def _chk_all(names, shape, *tensors):
+    """_chk(t, name, shape=shape) of every tensor that is not None, cheaply: small calls are
+    bound by the host."""
+    for t in tensors:
+        if t is not None and (t.shape != shape or t.dtype != torch.float32 or
+                              not t.is_contiguous() or not t.is_cuda):
+            for name, u in zip(names, tensors):
+                if u is t:
+                    _chk(t, name, shape=shape)
+
+
+@functools.lru_cache(maxsize=1024)
+def _ws_size(fn, *sizes):
+    """Workspace size functions whose result depends on the sizes alone."""
+    return max(call(fn, *sizes), 16)
 
 
 def workspace(nbytes: int, device=None) -> torch.Tensor:
@@ -153,8 +171,9 @@ def embedding_scaled_fwd(W, idx, scale=1.0):
     _chk(idx, "idx", torch.int64)
     V, D = W.shape
     N = idx.numel()
-    out = torch.empty((N, D), dtype=torch.float32, device=W.device)
-    call("ttk_embedding_scaled_fwd", _p(W), _p(idx), _p(out), N, D, V, scale, _s())
+    out = W.new_empty((N, D))
+    call("ttk_embedding_scaled_fwd", W.data_ptr(), idx.data_ptr(), out.data_ptr(), N, D, V, scale,
+         _s())
     return out
 
 
@@ -167,13 +186,14 @@ def embedding_scaled_bwd(dout, idx, V, scale=1.0, dW=None, accumulate=False):
     N, D = dout.shape
     if idx.numel() != N:
         raise ValueError(f"idx: expected {N} ids, got {idx.numel()}")
-    if dW is None:
-        dW = (torch.zeros if accumulate else torch.empty)((V, D), dtype=torch.float32,
-                                                          device=dout.device)
-    _chk(dW, "dW", shape=(V, D))
-    ws = workspace(call("ttk_embedding_scaled_bwd_workspace_size", N, D, V), dout.device)
-    call("ttk_embedding_scaled_bwd", _p(dout), _p(idx), _p(dW), int(accumulate), N, D, V, scale,
-         _p(ws), ws.numel(), _s())
+    if dW is not None:
+        _chk(dW, "dW", shape=(V, D))
+    else:
+        dW = dout.new_zeros((V, D)) if accumulate else dout.new_empty((V, D))
+    n = _ws_size("ttk_embedding_scaled_bwd_workspace_size", N, D, V)
+    ws = dout.new_empty(n, dtype=torch.uint8)
+    call("ttk_embedding_scaled_bwd", dout.data_ptr(), idx.data_ptr(), dW.data_ptr(),
+         int(accumulate), N, D, V, scale, ws.data_ptr(), n, _s())
     return dW
 
 
@@ -200,19 +220,16 @@ def residual_norm_fwd(x, b, w_post, w_next=None, gate=None, residual_scale=1.0, 
     y = rmsnorm(h, w_next). Without w_next y and rstd_next are None. gate: None, [1], [D],
     [R, 1] or [R, D]. With planes also the bf16x3 GEMM operand planes of y."""
     R, D = x.shape
-    for t, name, shape in ((x, "x", (R, D)), (b, "b", (R, D)), (w_post, "w_post", (D,)),
-                           (w_next, "w_next", (D,))):
-        if t is not None:
-            _chk(t, name, shape=shape)
+    _chk_all(("x", "b"), (R, D), x, b)
+    _chk_all(("w_post", "w_next"), (D,), w_post, w_next)
     kind = _gate_kind(gate, R, D)
-    h = torch.empty_like(x)
-    rstd = torch.empty((2, R), dtype=torch.float32, device=x.device)
-    y = None if w_next is None else torch.empty_like(x)
+    h, r1 = torch.empty_like(x), x.new_empty(R)
+    y, r2 = (None, None) if w_next is None else (torch.empty_like(x), x.new_empty(R))
     split = workspace(call("ttk_gemm_split_bytes", 1, R, D), x.device) if planes else None
-    call("ttk_residual_norm_fwd", _p(x), _p(b), _p(w_post), _p(gate), kind, _p(w_next), _p(h),
-         _p(y), _p(rstd), rstd.data_ptr() + 4 * R, _p(split), R, D, residual_scale, eps, _s())
-    out = (h, y, rstd[0], None if w_next is None else rstd[1])
-    return out + (split,) if planes else out
+    call("ttk_residual_norm_fwd", x.data_ptr(), b.data_ptr(), w_post.data_ptr(), _p(gate), kind,
+         _p(w_next), h.data_ptr(), _p(y), r1.data_ptr(), _p(r2), _p(split), R, D, residual_scale,
+         eps, _s())
+    return (h, y, r1, r2, split) if planes else (h, y, r1, r2)
 
 
 def residual_norm_bwd(dh, dy, h, b, w_post, w_next, rstd_post, rstd_next, gate=None,
@@ -222,32 +239,40 @@ def residual_norm_bwd(dh, dy, h, b, w_post, w_next, rstd_post, rstd_next, gate=N
     there). Output tensors that are given are added to; dgate is None without a gate, dw_next
     without dy."""
     R, D = b.shape
-    for t, name, shape in ((dh, "dh", (R, D)), (dy, "dy", (R, D)), (h, "h", (R, D)),
-                           (b, "b", (R, D)), (w_post, "w_post", (D,)), (w_next, "w_next", (D,)),
-                           (rstd_post, "rstd_post", (R,)), (rstd_next, "rstd_next", (R,)),
-                           (dx, "dx", (R, D)), (db, "db", (R, D)), (dw_post, "dw_post", (D,)),
-                           (dw_next, "dw_next", (D,)),
-                           (dgate, "dgate", None if gate is None else tuple(gate.shape))):
-        if t is not None:
-            _chk(t, name, shape=shape)
+    _chk_all(("dh", "dy", "h", "b", "dx", "db"), (R, D), dh, dy, h, b, dx, db)
+    _chk_all(("w_post", "w_next", "dw_post", "dw_next"), (D,), w_post, w_next, dw_post, dw_next)
+    _chk_all(("rstd_post", "rstd_next"), (R,), rstd_post, rstd_next)
     kind = _gate_kind(gate, R, D)
-    acc = (dx is not None) | (db is not None) << 1 | (dgate is not None) << 3
-    dx = torch.empty_like(b) if dx is None else dx
-    db = torch.empty_like(b) if db is None else db
-    # one flag covers both weights' gradients
-    acc |= (dw_post is not None or dw_next is not None) << 2
-    new_w = torch.zeros if acc & 4 else torch.empty
-    if dw_post is None:
-        dw_post = new_w(D, dtype=torch.float32, device=b.device)
-    if dw_next is None and dy is not None:
-        dw_next = new_w(D, dtype=torch.float32, device=b.device)
-    if dgate is None and gate is not None:
+    acc = 0
+    if dx is None:
+        dx = torch.empty_like(b)
+    else:
+        acc |= 1
+    if db is None:
+        db = torch.empty_like(b)
+    else:
+        acc |= 2
+    if dw_post is None and dw_next is None:
+        dw_post = torch.empty_like(w_post)
+        dw_next = None if dy is None else torch.empty_like(w_post)
+    else:  # one flag covers both weights' gradients
+        acc |= 4
+        dw_post = torch.zeros_like(w_post) if dw_post is None else dw_post
+        if dw_next is None and dy is not None:
+            dw_next = torch.zeros_like(w_post)
+    if gate is None:
+        dgate = None
+    elif dgate is None:
         dgate = torch.empty_like(gate)
-    ws = workspace(call("ttk_residual_norm_bwd_workspace_size", R, D), b.device)
-    call("ttk_residual_norm_bwd", _p(dh), _p(dy), _p(h), _p(b), _p(w_post), _p(gate), kind,
-         _p(w_next), _p(rstd_post), _p(rstd_next), _p(dx), _p(db), _p(dw_post),
-         _p(dw_next) if dy is not None else None, _p(dgate), acc, R, D, residual_scale, _p(ws),
-         ws.numel(), _s())
+    else:
+        _chk(dgate, "dgate", shape=gate.shape)
+        acc |= 8
+    n = _ws_size("ttk_residual_norm_bwd_workspace_size", R, D)
+    ws = b.new_empty(n, dtype=torch.uint8)
+    call("ttk_residual_norm_bwd", _p(dh), _p(dy), _p(h), b.data_ptr(), w_post.data_ptr(), _p(gate),
+         kind, _p(w_next), rstd_post.data_ptr(), _p(rstd_next), dx.data_ptr(), db.data_ptr(),
+         dw_post.data_ptr(), None if dy is None else dw_next.data_ptr(), _p(dgate), acc, R, D,
+         residual_scale, ws.data_ptr(), n, _s())
     return dx, db, dw_post, dw_next, dgate
 
 
@@ -276,14 +301,15 @@ def distill_loss(logits, teacher_ids, teacher_logits, targets=None, alpha=1.0, t
     if row_weight is not None:
         _chk(row_weight, "row_weight", shape=(N,))
     if want_grad and dlogits is None:
-        dlogits = torch.empty((N, C), dtype=torch.float32, device=logits.device)
-    loss = torch.empty(3, dtype=torch.float32, device=logits.device)
-    ws = workspace(call("ttk_distill_loss_workspace_size", N), logits.device)
-    call("ttk_distill_loss", _p(logits), max(logits.stride(0), C), _p(teacher_ids),
-         _p(teacher_logits), _TEACHER_TYPES[teacher_logits.dtype], K, _p(targets), _p(row_weight),
-         N, C, alpha, temperature, 1.0 / max(N, 1) if grad_scale is None else grad_scale, _p(loss),
-         _p(dlogits) if want_grad else None, max(dlogits.stride(0), C) if want_grad else 0, _p(ws),
-         ws.numel(), _s())
+        dlogits = logits.new_empty((N, C))
+    loss = logits.new_empty(3)
+    n = _ws_size("ttk_distill_loss_workspace_size", N)
+    ws = logits.new_empty(n, dtype=torch.uint8)
+    call("ttk_distill_loss", logits.data_ptr(), max(logits.stride(0), C), teacher_ids.data_ptr(),
+         teacher_logits.data_ptr(), _TEACHER_TYPES[teacher_logits.dtype], K, _p(targets),
+         _p(row_weight), N, C, alpha, temperature, 1.0 / max(N, 1) if grad_scale is None else
+         grad_scale, loss.data_ptr(), dlogits.data_ptr() if want_grad else None,
+         max(dlogits.stride(0), C) if want_grad else 0, ws.data_ptr(), n, _s())
     return loss, dlogits if want_grad else None
 
 
