@@ -168,3 +168,23 @@ def test_other_stream(cuda):
         got = K.embedding_scaled_bwd(dout + dout, ids, V, 1.5) + 0.0
     torch.cuda.current_stream().wait_stream(st)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("N,D,V", [(10, 4, 100), (3, 1, 4000), (60, 8, 900), (4096, 4, 1000),
+                                   (4097, 3, 2000), (5000, 1, 33), (70000, 2, 3000)])
+def test_small_tables(cuda, N, D, V):
+    """Tables of a few KB (one block zeroes them all) with tokens past the first 32."""
+    from tinytrain_b200 import kernels as K
+    g = torch.Generator(device=cuda).manual_seed(N)
+    for kind in ("uniform", "ends", "text"):
+        ids = tokens(kind, N, V, g, cuda)
+        dout = torch.randn(N, D, device=cuda, generator=g)
+        at, rows = ids.clamp(min=0), torch.where((ids >= 0)[:, None], dout.double(), 0.0)
+        ref = torch.zeros(V, D, device=cuda, dtype=torch.float64).index_add_(0, at, rows)
+        mag = torch.zeros(V, D, device=cuda, dtype=torch.float64).index_add_(0, at, rows.abs())
+        n = torch.bincount(at[ids >= 0], minlength=V).double()[:, None]
+        dW = torch.full((V, D), 9.0, device=cuda)  # written, not added to
+        K.embedding_scaled_bwd(dout, ids, V, 1.0, dW=dW)
+        assert ((dW.double() - ref).abs() <= (n + 2) * U * mag).all()
+        assert (dW[(n == 0).squeeze(1)] == 0).all()
+    assert status() == 0

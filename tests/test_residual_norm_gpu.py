@@ -217,3 +217,57 @@ def test_no_rows(cuda):
     _, _, dw1, _, _ = K.residual_norm_bwd(e, e, h, e, w, w, r1, r2, dw_post=have.clone())
     assert torch.equal(dw1, have)
     assert status() == 0
+
+
+@pytest.mark.parametrize("D", [128, 131, 2048])
+@pytest.mark.parametrize("kind", ["none", "column", "full"])
+def test_unaligned_tensors(cuda, D, kind):
+    """Tensors that start off a 16-byte boundary take another path, within the same bounds."""
+    from tinytrain_b200 import kernels as K
+    R, alpha, eps = 37, 0.5, 1e-5
+    s = make(R, D, kind, cuda)
+
+    def off(t):
+        return None if t is None else torch.cat([t.new_zeros(1), t.reshape(-1)])[1:].view(t.shape)
+
+    u = {k: off(v) for k, v in s.items()}
+    h, y, r1, r2 = K.residual_norm_fwd(u["x"], u["b"], u["w1"], u["w2"], gate=u["gate"],
+                                       residual_scale=alpha, eps=eps)
+    h64, hm, y64, ym, _, _ = forward64(s, alpha, eps)
+    c = D / 32 + 40
+    within(h, h64, hm, c, "h")
+    within(y, y64, ym, c, "y")
+    got = K.residual_norm_bwd(u["dh"], u["dy"], off(h), u["b"], u["w1"], u["w2"], r1, r2,
+                              gate=u["gate"], residual_scale=alpha)
+    ref = list(backward64(s, h, r1, r2, alpha, s["dh"], s["dy"]))
+    mag = list(backward64(s, h, r1, r2, alpha, s["dh"], s["dy"], positive=True))
+    for i, name in enumerate(("dx", "db", "dw_post", "dw_next")):
+        within(got[i], ref[i], mag[i], c + (R if i > 1 else 0), name)
+    if kind != "none":
+        within(got[4], to_gate(ref[4], s["gate"]), to_gate(mag[4], s["gate"]), c + R, "dgate")
+    assert status() == 0
+
+
+@pytest.mark.parametrize("R,D", [(5000, 66), (3001, 1111), (2003, 999), (1500, 2049), (700, 4095),
+                                 (600, 8191), (40000, 32)])
+def test_many_rows_of_odd_widths(cuda, R, D):
+    """More rows than the machine holds at once: every slot runs over several rows."""
+    from tinytrain_b200 import kernels as K
+    alpha, eps = 0.75, 1e-5
+    for kind in ("column", "full"):
+        s = make(R, D, kind, cuda)
+        h, y, r1, r2 = K.residual_norm_fwd(s["x"], s["b"], s["w1"], s["w2"], gate=s["gate"],
+                                           residual_scale=alpha, eps=eps)
+        h64, hm, y64, ym, _, _ = forward64(s, alpha, eps)
+        c = D / 32 + 40
+        within(h, h64, hm, c, "h")
+        within(y, y64, ym, c, "y")
+        got = K.residual_norm_bwd(s["dh"], s["dy"], h, s["b"], s["w1"], s["w2"], r1, r2,
+                                  gate=s["gate"], residual_scale=alpha)
+        ref = list(backward64(s, h, r1, r2, alpha, s["dh"], s["dy"]))
+        mag = list(backward64(s, h, r1, r2, alpha, s["dh"], s["dy"], positive=True))
+        for i, name in enumerate(("dx", "db", "dw_post", "dw_next")):
+            within(got[i], ref[i], mag[i], c + (R if i > 1 else 0), name)
+        within(got[4], to_gate(ref[4], s["gate"]), to_gate(mag[4], s["gate"]),
+               c + (R if kind == "column" else 0), "dgate")
+    assert status() == 0

@@ -818,6 +818,10 @@ int launch_rows(const Args& a, cudaStream_t st) {
     auto fits = [&](int ctas) {
         return words * 16 * 10 / 14 <= SMEM_SM / ctas - SMEM_CTA - list_bytes;
     };
+    // Few rows: one to a CTA, so as many threads to it as hold it (128 x 32000
+    // without a gradient, kernel alone: 13.6 us with 4 compute warps).
+    if (a.N <= 2 * 148 && a.C > NARROW_MAX)
+        return launch<TWO, 14, 3, 2>(a, cut, list_bytes, st);
     if (fits(8))
         return launch<TWO, 2, 4, 8>(a, cut, list_bytes, st);
     if (fits(4) || !a.dlogits)

@@ -4,10 +4,16 @@
 //   dW[v,:] (+)= scale * sum_{i: t_i = v} dout[i,:]
 // The gradient sorts the positions by token, so every row of dW is written
 // once, by one summation in a fixed order: no floating-point atomics.
+//
+// Both are bound by HBM. Lookup, 32768 x 2048 of 32000 rows: 57 us, 6.1 TB/s of
+// the rows read and written. Gradient of the same, dW written: 100 us, 5.3 TB/s
+// of dout read and dW written (the sort beside the zeroing of the rows without
+// a token 40, the sums 48, the runs that cross chunks 10).
 #include <cuda_runtime.h>
 #include <stdint.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "pdl.cuh"
 #include "ttk_common.cuh"
@@ -74,55 +80,81 @@ __global__ void __launch_bounds__(256) lookup_kernel(const float* __restrict__ W
 // ---------------------------------------------------------------- sorting --
 // (token, position) pairs in ascending order, tokens outside [0, V) as V, so
 // last. Two ways:
-//   rank_kernel, up to 8192 positions: every pair is packed into 32 bits, and
+//   rank_kernel, up to 4096 positions: every pair is packed into 32 bits, and
 //     a pair's place is the number of smaller ones, counted by one warp over
-//     all of them in shared memory. No step waits for another.
+//     all of them in shared memory. No step waits for another (a gradient of
+//     2000 x 768 of 32000 rows: 25.4 us against 28.5 by the other, 4096 x 768:
+//     30.1 against 30.9, 8192 x 768: 41 against 34).
 //   radix_kernel: a stable radix sort by one cluster of 8 blocks, 8 bits a
 //     pass. Each warp owns a contiguous run of the pairs: it counts its digits,
 //     the counts are scanned over the warps of the block and over the blocks
 //     (through distributed shared memory), and the warp writes its pairs in
-//     order.
+//     order (24 us for 32768 positions by itself). Up to 65536 positions the pairs stay in the cluster's shared memory
+//     between the passes (LOCAL): through global memory the passes would wait
+//     behind the zeroing blocks' writes.
 // Neither needs the whole machine; when dW is written (not added to), the
 // launch's other blocks meanwhile zero the rows of tokens that do not occur.
-// Each owns a range of rows and marks the range's tokens in a bitmap of its
-// own by reading all the ids (from L2), so it waits for nobody.
+// Each owns some of the rows and marks their tokens in a bitmap of its own by
+// reading all the ids (from L2), so it waits for nobody.
 constexpr int SORT_CTAS = 8;
 constexpr int SORT_THREADS = 1024;
 constexpr int SORT_WARPS = SORT_THREADS / 32;
 constexpr int RADIX = 256;
-constexpr int64_t ROWS_A_ROUND = RADIX * SORT_WARPS * 32;  // rows one bitmap covers
-constexpr int RANK_BITS = 13;
+constexpr int64_t LOCAL_MAX = 65536;  // 2 x 64 KB of pairs a block
+constexpr uint32_t BITMAP_WORDS = RADIX * SORT_WARPS;
+constexpr int RANK_BITS = 12;
 constexpr int64_t RANK_MAX = 1 << RANK_BITS;
 constexpr int RANK_THREADS = 256;
 constexpr int RANK_KEYS = 4;  // places a warp counts at once
 
-// Rows [v0, v1) of dW that no id names are set to zero. VEC as above.
+// The rows of dW that no id names are set to zero, in groups of 32: groups z,
+// z + nz, z + 2 nz, ... here (frequent tokens have low ids in most vocabularies,
+// so ranges of rows would be uneven). VEC as above.
 template <int VEC>
-__device__ void zero_absent(const int64_t* __restrict__ idx, int64_t N, int64_t v0, int64_t v1,
-                            float* __restrict__ dW, int64_t D, uint32_t* __restrict__ bits) {
+__device__ void zero_absent(const int64_t* __restrict__ idx, int64_t N, int64_t V, uint32_t z,
+                            uint32_t nz, float* __restrict__ dW, int64_t D,
+                            uint32_t* __restrict__ bits) {
     using T = typename Vec<VEC>::T;
     const int64_t words = D / VEC;
-    for (int64_t a = v0; a < v1; a += ROWS_A_ROUND) {
-        const int64_t e = min(v1, a + ROWS_A_ROUND);
+    const uint32_t groups = static_cast<uint32_t>((V + 31) / 32);
+    const uint32_t mine = z < groups ? (groups - z + nz - 1) / nz : 0;
+    const uint32_t inv = 0xffffffffu / nz;
+    for (uint32_t a = 0; a < mine; a += BITMAP_WORDS) {
+        const uint32_t n = min(mine - a, BITMAP_WORDS);
         __syncthreads();
-        for (int64_t i = threadIdx.x; i < (e - a + 31) / 32; i += blockDim.x)
+        for (uint32_t i = threadIdx.x; i < n; i += blockDim.x)
             bits[i] = 0;
         __syncthreads();
-#pragma unroll 4
-        for (int64_t i = threadIdx.x; i < N; i += blockDim.x) {
-            const int64_t t = idx[i];
-            if (t >= a && t < e)
-                atomicOr(bits + ((t - a) >> 5), 1u << ((t - a) & 31));
+        for (int64_t i0 = threadIdx.x; i0 < N; i0 += 8 * static_cast<int64_t>(blockDim.x)) {
+            int64_t t[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                t[j] = i0 + j * static_cast<int64_t>(blockDim.x) < N ? idx[i0 + j * blockDim.x] : -1;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                // group / nz, by the reciprocal's lower bound
+                const uint32_t g = static_cast<uint32_t>(t[j]) >> 5;
+                uint32_t q = __umulhi(g, inv), rest = g - q * nz;
+                if (rest >= nz)
+                    rest -= nz, ++q;
+                const uint32_t bit = 1u << (t[j] & 31);
+                // frequent tokens are marked once: atomics on one word queue up
+                if (t[j] >= 0 && t[j] < V && rest == z && q - a < n &&
+                    !(*const_cast<volatile uint32_t*>(bits + (q - a)) & bit))
+                    atomicOr(bits + (q - a), bit);
+            }
         }
         __syncthreads();
         const int lane = threadIdx.x & 31;
-        for (int64_t v = a + (threadIdx.x >> 5); v < e; v += blockDim.x >> 5)
-            if (!((bits[(v - a) >> 5] >> ((v - a) & 31)) & 1u)) {
+        for (uint32_t r = threadIdx.x >> 5; r < 32 * n; r += blockDim.x >> 5) {
+            const int64_t v = (static_cast<int64_t>(a + (r >> 5)) * nz + z) * 32 + (r & 31);
+            if (v < V && !((bits[r >> 5] >> (r & 31)) & 1u)) {
                 T* row = reinterpret_cast<T*>(dW + v * D);
 #pragma unroll 4
                 for (int64_t c = lane; c < words; c += 32)
                     row[c] = zero<T>();
             }
+        }
     }
 }
 
@@ -131,12 +163,12 @@ __global__ void __launch_bounds__(RANK_THREADS)
     rank_kernel(const int64_t* __restrict__ idx, int N, int64_t V, int sorters,
                 uint64_t* __restrict__ keys, uint32_t* __restrict__ count, float* __restrict__ dW,
                 int64_t D) {
-    __shared__ __align__(16) uint32_t pairs[RANK_MAX];
-    static_assert(RANK_MAX * 32 >= ROWS_A_ROUND, "the pairs' memory holds a bitmap");
+    // the pairs, or a zeroing block's bitmap
+    __shared__ __align__(16) uint32_t pairs[RANK_MAX > BITMAP_WORDS ? RANK_MAX : BITMAP_WORDS];
     grid_wait();
     if (static_cast<int>(blockIdx.x) >= sorters) {
-        const int64_t nz = gridDim.x - sorters, z = blockIdx.x - sorters;
-        zero_absent<VEC>(idx, N, V * z / nz, V * (z + 1) / nz, dW, D, pairs);
+        const uint32_t nz = gridDim.x - sorters, z = blockIdx.x - sorters;
+        zero_absent<VEC>(idx, N, V, z, nz, dW, D, pairs);
         return;
     }
     if (blockIdx.x == 0 && threadIdx.x == 0)
@@ -186,19 +218,24 @@ __device__ __forceinline__ uint32_t ld_cluster(const uint32_t* p, uint32_t rank)
     return v;
 }
 
-template <int VEC>
+__device__ __forceinline__ void st_cluster(uint64_t* p, uint32_t rank, uint64_t v) {
+    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(smem_in_cta(p, rank)), "l"(v) : "memory");
+}
+
+template <int VEC, bool LOCAL>
 __global__ void __cluster_dims__(SORT_CTAS, 1, 1) __launch_bounds__(SORT_THREADS)
     radix_kernel(const int64_t* __restrict__ idx, int64_t N, int64_t V, int passes,
                  uint64_t* __restrict__ bufa, uint64_t* __restrict__ bufb,
                  uint32_t* __restrict__ count, float* __restrict__ dW, int64_t D) {
+    extern __shared__ __align__(16) uint64_t pairs[];  // LOCAL: [2][pairs of a block]
     __shared__ uint32_t hist[SORT_WARPS][RADIX];
     __shared__ uint32_t total[RADIX];
     __shared__ uint32_t wsum[8];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     grid_wait();
     if (blockIdx.x >= SORT_CTAS) {  // whole clusters
-        const int64_t nz = gridDim.x - SORT_CTAS, z = blockIdx.x - SORT_CTAS;
-        zero_absent<VEC>(idx, N, V * z / nz, V * (z + 1) / nz, dW, D, &hist[0][0]);
+        const uint32_t nz = gridDim.x - SORT_CTAS, z = blockIdx.x - SORT_CTAS;
+        zero_absent<VEC>(idx, N, V, z, nz, dW, D, &hist[0][0]);
         return;
     }
     const uint32_t rank = cluster_ctarank();
@@ -208,15 +245,34 @@ __global__ void __cluster_dims__(SORT_CTAS, 1, 1) __launch_bounds__(SORT_THREADS
     const int64_t per = ((N + nwarps - 1) / nwarps + 31) / 32 * 32;
     const int64_t lo = (static_cast<int64_t>(rank) * SORT_WARPS + warp) * per;
     const int64_t hi = min(N, lo + per);
+    const int64_t block = per * SORT_WARPS, mine = rank * block;  // this block's pairs
+    auto first = [&](int64_t i) -> uint64_t {
+        const int64_t t = idx[i];
+        const bool live = t >= 0 && t < V;
+        if (!live && t != -1)
+            report(kErrBadIndex);
+        return (static_cast<uint64_t>(live ? t : V) << 32) | static_cast<uint64_t>(i);
+    };
+    if (LOCAL) {  // pass 0 reads the second half, as every even pass
+#pragma unroll 4
+        for (int64_t i = lo + lane; i < hi; i += 32)
+            pairs[block + i - mine] = first(i);
+        __syncwarp();
+    }
     auto load = [&](int pass, int64_t i) -> uint64_t {
-        if (pass == 0) {
-            const int64_t t = idx[i];
-            const bool live = t >= 0 && t < V;
-            if (!live && t != -1)
-                report(kErrBadIndex);
-            return (static_cast<uint64_t>(live ? t : V) << 32) | static_cast<uint64_t>(i);
-        }
+        if (LOCAL)
+            return pairs[((pass & 1) ? 0 : block) + i - mine];
+        if (pass == 0)
+            return first(i);
         return __ldcg(reinterpret_cast<const unsigned long long*>((pass & 1) ? bufa : bufb) + i);
+    };
+    auto store = [&](int pass, uint32_t place, uint64_t key) {
+        if (LOCAL && pass + 1 < passes) {
+            const uint32_t to = place / static_cast<uint32_t>(block);
+            st_cluster(pairs + ((pass & 1) ? block : 0) + (place - to * block), to, key);
+        } else {
+            ((pass & 1) ? bufb : bufa)[place] = key;
+        }
     };
     for (int pass = 0; pass < passes; ++pass) {
         const int shift = 32 + 8 * pass;
@@ -267,11 +323,11 @@ __global__ void __cluster_dims__(SORT_CTAS, 1, 1) __launch_bounds__(SORT_THREADS
             uint32_t base = scan - all + before;
             for (int w = 0; w < warp; ++w)
                 base += wsum[w];
+#pragma unroll
             for (int w = 0; w < SORT_WARPS; ++w)
                 hist[w][tid] += base;
         }
         __syncthreads();
-        uint64_t* dst = (pass & 1) ? bufb : bufa;
         for (int64_t i = lo + lane; i - lane < hi; i += 32) {
             const bool ok = i < hi;
             const uint64_t key = ok ? load(pass, i) : 0;
@@ -279,13 +335,14 @@ __global__ void __cluster_dims__(SORT_CTAS, 1, 1) __launch_bounds__(SORT_THREADS
             const uint32_t same = __match_any_sync(~0u, d);
             const uint32_t below = __popc(same & ((1u << lane) - 1));
             if (ok)
-                dst[hist[warp][d] + below] = key;
+                store(pass, hist[warp][d] + below, key);
             __syncwarp();
             if (ok && below == 0)
                 hist[warp][d] += __popc(same);
             __syncwarp();
         }
-        __threadfence();
+        if (!LOCAL)
+            __threadfence();
         cluster_sync();
     }
 }
@@ -309,7 +366,7 @@ __global__ void __launch_bounds__(256)
     chunk_kernel(const uint64_t* __restrict__ keys, int64_t N, int L, const float* __restrict__ dout,
                  float* __restrict__ dW, int accumulate, int64_t D, int64_t V, float scale,
                  float* __restrict__ part, uint32_t* __restrict__ count,
-                 uint32_t* __restrict__ list) {
+                 uint2* __restrict__ list) {
     using T = typename Vec<VEC>::T;
     __shared__ uint64_t s_key[MAX_L + 2];  // the chunk's keys, its neighbours on both sides
     const int64_t first = static_cast<int64_t>(blockIdx.x) * L;
@@ -353,7 +410,7 @@ __global__ void __launch_bounds__(256)
             if (earlier || more) {
                 slots[earlier ? 0 : words] = acc;
                 if (!earlier && c == 0)
-                    list[atomicAdd(count, 1u)] = blockIdx.x;
+                    list[atomicAdd(count, 1u)] = make_uint2(blockIdx.x, t);
             } else {
                 T* d = reinterpret_cast<T*>(dW) + static_cast<int64_t>(t) * words + c;
                 const T r = times(acc, scale);
@@ -365,52 +422,51 @@ __global__ void __launch_bounds__(256)
     }
 }
 
-// Runs that cross chunks: a block takes one listed chunk and 32 words of the
-// row at a time, and adds the partial sums in eight interleaved sequences of
-// chunks, then those in order.
-constexpr int JOIN_WAYS = 8;
-constexpr int JOIN_THREADS = 32 * JOIN_WAYS;
+// Runs that cross chunks: a block takes one listed (chunk, token) and 256 words
+// of the row at a time, and adds the partial sums in two interleaved sequences
+// of chunks, then those two.
+constexpr int JOIN_WORDS = 256;
+constexpr int JOIN_THREADS = 2 * JOIN_WORDS;
 template <int VEC>
 __global__ void __launch_bounds__(JOIN_THREADS)
     join_kernel(const uint64_t* __restrict__ keys, int64_t N, int L, float* __restrict__ dW,
                 int accumulate, int64_t D, float scale, const float* __restrict__ part,
-                const uint32_t* __restrict__ count, const uint32_t* __restrict__ list) {
+                const uint32_t* __restrict__ count, const uint2* __restrict__ list) {
     using T = typename Vec<VEC>::T;
-    __shared__ T s_part[JOIN_WAYS][32];
-    const int lane = threadIdx.x & 31, way = threadIdx.x >> 5;
-    const int64_t words = D / VEC, tiles = (words + 31) / 32;
+    __shared__ T s_part[JOIN_WORDS];
+    const int at = threadIdx.x % JOIN_WORDS, way = threadIdx.x / JOIN_WORDS;
+    const int64_t words = D / VEC, tiles = (words + JOIN_WORDS - 1) / JOIN_WORDS;
     grid_wait();
     const int64_t items = static_cast<int64_t>(*count) * tiles;
     for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const int64_t chunk = list[item / tiles], c = item % tiles * 32 + lane;
-        const uint32_t t = key_token(keys[(chunk + 1) * L - 1]);
-        // chunks whose first run is this token's
-        int64_t more = 0;
+        const uint2 run = list[item / tiles];
+        const int64_t chunk = run.x, c = item % tiles * JOIN_WORDS + at;
+        const T* p = reinterpret_cast<const T*>(part) + c;
+        T* d = reinterpret_cast<T*>(dW) + static_cast<int64_t>(run.y) * words + c;
+        // on their way while the run's length is found: its first two partial
+        // sums (there are two at least) and the row to add to
+        T acc = zero<T>(), old = zero<T>();
+        if (c < words) {
+            acc = p[(2 * (chunk + way) + (way ? 0 : 1)) * words];
+            if (accumulate && way == 0)
+                old = *d;
+        }
+        int64_t more = 0;  // chunks whose first run is this token's
         int found;
         do {
-            const int64_t p = (chunk + 1 + more + threadIdx.x) * L;
-            found = __syncthreads_count(p < N && key_token(keys[p]) == t);
+            const int64_t k = (chunk + 1 + more + threadIdx.x) * L;
+            found = __syncthreads_count(k < N && key_token(keys[k]) == run.y);
             more += found;
         } while (found == JOIN_THREADS);
-        const T* p = reinterpret_cast<const T*>(part) + c;
-        T acc = zero<T>();
-        if (c < words) {
-            if (way == 0)
-                acc = p[(2 * chunk + 1) * words];
+        if (c < words)
 #pragma unroll 8
-            for (int64_t k = chunk + 1 + way; k <= chunk + more; k += JOIN_WAYS)
+            for (int64_t k = chunk + 2 + way; k <= chunk + more; k += 2)
                 acc = plus(acc, p[2 * k * words]);
-        }
-        s_part[way][lane] = acc;
+        if (way)
+            s_part[at] = acc;
         __syncthreads();
-        if (way == 0 && c < words) {
-#pragma unroll
-            for (int i = 1; i < JOIN_WAYS; ++i)
-                acc = plus(acc, s_part[i][lane]);
-            T* d = reinterpret_cast<T*>(dW) + static_cast<int64_t>(t) * words + c;
-            const T r = times(acc, scale);
-            *d = accumulate ? plus(*d, r) : r;
-        }
+        if (way == 0 && c < words)
+            *d = plus(times(plus(acc, s_part[at]), scale), old);
     }
 }
 
@@ -438,11 +494,44 @@ Plan plan(int64_t N, int64_t D, bool aligned) {
     return p;
 }
 
+// Clusters of the radix kernel that are resident at once, the sort's among them
+// (more of them would leave some for a second round: 32768 x 2048 took 120 us
+// with 16 clusters and 103 us with 14).
+template <int VEC>
+int resident_clusters() {
+    static std::atomic<int> known[16];  // by device
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev >= 16)
+        dev = 0;
+    int n = known[dev].load(std::memory_order_relaxed);
+    if (n)
+        return n;
+    constexpr int smem = 128 * 1024;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(SORT_CTAS);
+    cfg.blockDim = dim3(SORT_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = SORT_CTAS;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaFuncSetAttribute(radix_kernel<VEC, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             smem) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, radix_kernel<VEC, true>, &cfg) != cudaSuccess || n < 2) {
+        cudaGetLastError();
+        n = 2;
+    }
+    known[dev].store(n, std::memory_order_relaxed);
+    return n;
+}
+
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // Workspace: two key buffers, the list's count, the list, the partial rows.
 size_t workspace_bytes(const Plan& p, int64_t D) {
-    return 2 * p.keys + 16 + align16(static_cast<size_t>(p.chunks) * 4) +
+    return 2 * p.keys + 16 + align16(static_cast<size_t>(p.chunks) * 8) +
            static_cast<size_t>(p.chunks) * 2 * D * sizeof(float);
 }
 
@@ -452,9 +541,9 @@ int backward(const float* dout, const int64_t* idx, float* dW, int accumulate, i
     uint64_t* bufa = reinterpret_cast<uint64_t*>(ws);
     uint64_t* bufb = reinterpret_cast<uint64_t*>(ws + p.keys);
     uint32_t* count = reinterpret_cast<uint32_t*>(ws + 2 * p.keys);
-    uint32_t* list = count + 4;
+    uint2* list = reinterpret_cast<uint2*>(count + 4);
     float* part = reinterpret_cast<float*>(ws + 2 * p.keys + 16 +
-                                           align16(static_cast<size_t>(p.chunks) * 4));
+                                           align16(static_cast<size_t>(p.chunks) * 8));
     const uint64_t* keys = bufa;
     int rc;
     if (N <= RANK_MAX && V < (1ll << (32 - RANK_BITS)) - 1) {
@@ -469,12 +558,25 @@ int backward(const float* dout, const int64_t* idx, float* dW, int accumulate, i
         int passes = 1;
         while (passes < 4 && (V >> (8 * passes)))
             ++passes;
-        // 64 KB of rows a zeroing block, all clusters resident at once
-        const int64_t zeros =
-            accumulate ? 0 : std::min<int64_t>(15, V * D / (16384 * SORT_CTAS) + 1) * SORT_CTAS;
-        rc = launch_pdl("embedding_scaled_bwd sort", radix_kernel<VEC>,
-                        dim3(static_cast<unsigned>(SORT_CTAS + zeros)), SORT_THREADS, 0, st, idx, N,
-                        V, passes, bufa, bufb, count, dW, D);
+        // 64 KB of rows a zeroing block at least
+        const int64_t zeros = accumulate ? 0
+                                         : std::min<int64_t>(resident_clusters<VEC>() - 1,
+                                                             V * D / (16384 * SORT_CTAS) + 1) *
+                                               SORT_CTAS;
+        const dim3 grid(static_cast<unsigned>(SORT_CTAS + zeros));
+        if (N <= LOCAL_MAX) {
+            const int64_t per = ((N + SORT_CTAS * SORT_WARPS - 1) / (SORT_CTAS * SORT_WARPS) + 31) / 32 * 32;
+            const size_t smem = static_cast<size_t>(per) * SORT_WARPS * 2 * sizeof(uint64_t);
+            const cudaError_t e = cudaFuncSetAttribute(
+                radix_kernel<VEC, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, 128 * 1024);
+            if (e != cudaSuccess)
+                return check_cuda(e, "embedding_scaled_bwd sort");
+            rc = launch_pdl("embedding_scaled_bwd sort", radix_kernel<VEC, true>, grid,
+                            SORT_THREADS, smem, st, idx, N, V, passes, bufa, bufb, count, dW, D);
+        } else {
+            rc = launch_pdl("embedding_scaled_bwd sort", radix_kernel<VEC, false>, grid,
+                            SORT_THREADS, 0, st, idx, N, V, passes, bufa, bufb, count, dW, D);
+        }
         keys = (passes & 1) ? bufa : bufb;
     }
     if (!rc)
@@ -482,13 +584,13 @@ int backward(const float* dout, const int64_t* idx, float* dW, int accumulate, i
                         dim3(static_cast<unsigned>(p.chunks), static_cast<unsigned>(p.tiles)),
                         p.threads, 0, st, keys, N, p.L, dout, dW, accumulate, D, V, scale, part,
                         count, list);
-    const int64_t items = p.chunks * ((p.words + 31) / 32);  // at most
+    const int64_t items = p.chunks * ((p.words + JOIN_WORDS - 1) / JOIN_WORDS);  // at most
     if (!rc)
         rc = launch_pdl("embedding_scaled_bwd join", join_kernel<VEC>,
-                        dim3(static_cast<unsigned>(std::min<int64_t>(items, 148 * 8))), JOIN_THREADS,
+                        dim3(static_cast<unsigned>(std::min<int64_t>(items, 148 * 4))), JOIN_THREADS,
                         0, st, keys, N, p.L, dW, accumulate, D, scale,
                         static_cast<const float*>(part), static_cast<const uint32_t*>(count),
-                        static_cast<const uint32_t*>(list));
+                        static_cast<const uint2*>(list));
     return rc;
 }
 

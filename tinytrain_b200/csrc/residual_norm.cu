@@ -68,71 +68,80 @@ struct Bwd {
     float alpha;
 };
 
-// One thread's share of a row: NV words of VEC consecutive floats (VEC = 4
-// needs D % 4 == 0 and aligned tensors), word j at (j * TPR + t) * VEC.
-template <int VEC, int NV>
+// One thread's share of a row: NV words of four floats, word j at 16-byte word
+// j * TPR + t of the row. Rows of a width that is no multiple of four (ODD) begin
+// `off` floats into their first word; the words that a row shares with its
+// neighbours belong to it in part. A slot's rows are chosen to have one `off`,
+// so that a thread's columns stay the same.
+template <int NV, bool ODD>
 struct Cols {
-    static constexpr int E = VEC * NV;
-    int64_t c[NV];
-    bool in[NV];
-    __device__ __forceinline__ Cols(int t, int tpr, int64_t D) {
+    static constexpr int E = 4 * NV;
+    int w[NV];  // word of the row
+    int c[NV];  // its first column (negative in the first word of an odd row)
+    bool in[NV], full[NV];
+    int D;
+    __device__ __forceinline__ Cols(int t, int tpr, int64_t width, int off)
+        : D(static_cast<int>(width)) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            c[j] = (static_cast<int64_t>(j) * tpr + t) * VEC;
+            w[j] = j * tpr + t;
+            c[j] = 4 * w[j] - (ODD ? off : 0);
             in[j] = c[j] < D;
+            full[j] = ODD ? c[j] >= 0 && c[j] + 4 <= D : in[j];
         }
     }
-    __device__ __forceinline__ void load(float (&v)[E], const float* row, bool ok) const {
+    // columns of p, whose alignment is the row's (ALIGNED) or any
+    template <bool ALIGNED>
+    __device__ __forceinline__ void load(float (&v)[E], const float* p, bool ok) const {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            if constexpr (VEC == 4) {
-                const float4 q = ok && in[j] ? *reinterpret_cast<const float4*>(row + c[j])
-                                             : make_float4(0.f, 0.f, 0.f, 0.f);
-                v[4 * j] = q.x, v[4 * j + 1] = q.y, v[4 * j + 2] = q.z, v[4 * j + 3] = q.w;
-            } else {
-                v[j] = ok && in[j] ? row[c[j]] : 0.0f;
-            }
+            float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (ok && full[j] && (ALIGNED || !ODD))
+                q = *reinterpret_cast<const float4*>(p + c[j]);
+            v[4 * j] = q.x, v[4 * j + 1] = q.y, v[4 * j + 2] = q.z, v[4 * j + 3] = q.w;
+            if (ODD && ok && in[j] && !(ALIGNED && full[j]))
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (c[j] + u >= 0 && c[j] + u < D)
+                        v[4 * j + u] = p[c[j] + u];
         }
     }
-    __device__ __forceinline__ void store(float* row, const float (&v)[E]) const {
+    template <bool ALIGNED>
+    __device__ __forceinline__ void store(float* p, const float (&v)[E]) const {
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
-            if (in[j]) {
-                if constexpr (VEC == 4)
-                    *reinterpret_cast<float4*>(row + c[j]) =
-                        make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-                else
-                    row[c[j]] = v[j];
-            }
+        for (int j = 0; j < NV; ++j) {
+            if (full[j] && (ALIGNED || !ODD))
+                *reinterpret_cast<float4*>(p + c[j]) =
+                    make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+            if (ODD && in[j] && !(ALIGNED && full[j]))
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (c[j] + u >= 0 && c[j] + u < D)
+                        p[c[j] + u] = v[4 * j + u];
+        }
     }
     __device__ __forceinline__ void add_store(float* row, const float (&v)[E], bool add) const {
         if (!add)
-            return store(row, v);
+            return store<true>(row, v);
         float o[E];
-        load(o, row, true);
+        load<true>(o, row, true);
 #pragma unroll
         for (int i = 0; i < E; ++i)
             o[i] += v[i];
-        store(row, o);
+        store<true>(row, o);
     }
-    // hi and lo planes of v, `plane` elements apart
+    // hi and lo planes of v, `plane` elements apart (widths of whole words)
     __device__ __forceinline__ void store_split(__nv_bfloat16* row, int64_t plane,
                                                 const float (&v)[E]) const {
 #pragma unroll
         for (int j = 0; j < NV; ++j)
             if (in[j]) {
-                __nv_bfloat16 hi[VEC], lo[VEC];
+                __nv_bfloat16 hi[4], lo[4];
 #pragma unroll
-                for (int u = 0; u < VEC; ++u)
-                    split_bf16(v[VEC * j + u], hi[u], lo[u]);
-                if constexpr (VEC == 4) {
-                    *reinterpret_cast<uint2*>(row + c[j]) = *reinterpret_cast<const uint2*>(hi);
-                    *reinterpret_cast<uint2*>(row + plane + c[j]) =
-                        *reinterpret_cast<const uint2*>(lo);
-                } else {
-                    row[c[j]] = hi[0];
-                    row[plane + c[j]] = lo[0];
-                }
+                for (int u = 0; u < 4; ++u)
+                    split_bf16(v[4 * j + u], hi[u], lo[u]);
+                *reinterpret_cast<uint2*>(row + c[j]) = *reinterpret_cast<const uint2*>(hi);
+                *reinterpret_cast<uint2*>(row + plane + c[j]) = *reinterpret_cast<const uint2*>(lo);
             }
     }
 };
@@ -175,98 +184,81 @@ __device__ __forceinline__ bool row_sum(float (&v)[N], float* red, int slot, int
     return all != 0;
 }
 
-// A row of a tensor [R, D] as a bulk copy moves it: 16-byte pieces. `off` is
-// the row's start within its first piece, the copy covers elements [head,
-// tail) of the row. Pieces that the row shares with its neighbours are copied
-// whole; at the tensor's two ends, where there is no neighbour, the few
-// elements of such a piece are left to plain loads.
-struct Span {
-    const float* src;
-    int off, head, tail;
-    uint32_t bytes;
-};
-
-template <int VEC>
-__device__ __forceinline__ Span span_of(const float* base, int64_t row, int64_t R, int64_t D) {
-    const float* p = base + row * D;
-    if constexpr (VEC == 4)
-        return Span{p, 0, 0, static_cast<int>(D), static_cast<uint32_t>(D) * 4u};
-    Span s;
-    s.off = static_cast<int>((reinterpret_cast<uintptr_t>(p) & 15) >> 2);
-    s.head = -s.off;
-    if (s.off && row == 0)
-        s.head += 4;
-    s.tail = static_cast<int>((D + s.off + 3) / 4 * 4) - s.off;
-    if (s.tail > D && row == R - 1)
-        s.tail -= 4;
-    s.src = p + s.head;
-    s.bytes = s.tail > s.head ? static_cast<uint32_t>(s.tail - s.head) * 4u : 0u;
-    return s;
-}
-
 constexpr int MAX_STAGES = 4;
 constexpr int MAX_SLOTS = 8;
 
 // The slot's stages of NT rows (one per tensor; a null tensor is skipped and
-// reads as zeros), `pitch` floats each.
-template <int VEC, int NV, int NT>
+// reads as zeros), `pitch` floats each. A bulk copy moves a row's words whole,
+// with what they hold of its neighbours; the last word of the last row of a
+// tensor has no neighbour behind it and is left to plain loads.
+template <int NV, bool ODD, int NT>
 struct Feed {
-    static constexpr int E = VEC * NV;
+    static constexpr int E = 4 * NV;
     const float* t[NT];
     float* buf;  // [stages][NT][pitch]
     uint64_t* bar;
     int64_t R, D;
-    int pitch, stages;
+    int off, pitch;
 
     __device__ __forceinline__ void issue(int stage, int64_t row) const {
-        uint32_t bytes = 0;
+        uint32_t bytes = static_cast<uint32_t>(D) * 4u;
+        if (ODD) {
+            int words = static_cast<int>((off + D + 3) / 4);
+            if (row == R - 1 && (off + D) % 4)
+                --words;
+            bytes = static_cast<uint32_t>(words) * 16u;
+        }
+        uint32_t total = 0;
 #pragma unroll
         for (int i = 0; i < NT; ++i)
-            if (t[i])
-                bytes += span_of<VEC>(t[i], row, R, D).bytes;
-        mbar_arrive_expect_tx(bar + stage, bytes);
+            total += t[i] ? bytes : 0u;
+        mbar_arrive_expect_tx(bar + stage, total);
 #pragma unroll
         for (int i = 0; i < NT; ++i)
-            if (t[i]) {
-                const Span s = span_of<VEC>(t[i], row, R, D);
-                if (s.bytes)
-                    bulk_load(buf + (stage * NT + i) * pitch + s.off + s.head, s.src, s.bytes,
-                              bar + stage);
-            }
+            if (t[i] && bytes)
+                bulk_load(buf + (stage * NT + i) * pitch, t[i] + row * D - (ODD ? off : 0), bytes,
+                          bar + stage);
     }
     __device__ __forceinline__ void read(float (&v)[E], int i, int stage, int64_t row,
-                                         const Cols<VEC, NV>& cols) const {
-        const float* b = buf + (stage * NT + i) * pitch;
-        if (VEC == 4 || !t[i])
-            return cols.load(v, b, t[i] != nullptr);
-        const Span s = span_of<VEC>(t[i], row, R, D);
+                                         const Cols<NV, ODD>& cols) const {
+        const float4* b = reinterpret_cast<const float4*>(buf + (stage * NT + i) * pitch);
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
-            v[j] = !cols.in[j] ? 0.0f
-                   : cols.c[j] >= s.head && cols.c[j] < s.tail ? b[s.off + cols.c[j]]
-                                                               : t[i][row * D + cols.c[j]];
+        for (int j = 0; j < NV; ++j) {
+            const float4 q = t[i] && cols.in[j] ? b[cols.w[j]] : make_float4(0.f, 0.f, 0.f, 0.f);
+            v[4 * j] = q.x, v[4 * j + 1] = q.y, v[4 * j + 2] = q.z, v[4 * j + 3] = q.w;
+            if (ODD && t[i] && cols.in[j] && !cols.full[j])  // a word shared with a neighbour
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int c = cols.c[j] + u;
+                    if (c < 0 || c >= cols.D)
+                        v[4 * j + u] = 0.0f;
+                    else if (row == R - 1)
+                        v[4 * j + u] = t[i][row * D + c];
+                }
+        }
     }
 };
 
-template <int VEC, int NV, bool FULL>
+template <int NV, bool ODD, bool FULL>
 __global__ void __launch_bounds__(512) fwd_rows_kernel(const Fwd a, int tpr, int pitch, int stages) {
-    constexpr int E = VEC * NV, NT = FULL ? 3 : 2;
+    constexpr int E = 4 * NV, NT = FULL ? 3 : 2;
     extern __shared__ __align__(16) float smem[];
     __shared__ float red[2][MAX_WARPS];
     __shared__ __align__(8) uint64_t bars[MAX_SLOTS * MAX_STAGES];
     const int slot = threadIdx.x / tpr, slots = blockDim.x / tpr;
     const bool lead = threadIdx.x == slot * tpr;
     const int64_t D = a.D;
-    const Cols<VEC, NV> cols(threadIdx.x - slot * tpr, tpr, D);
-    Feed<VEC, NV, NT> feed;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * slots;
+    int64_t row = static_cast<int64_t>(blockIdx.x) * slots + slot;
+    const int off = ODD ? static_cast<int>((row * D) & 3) : 0;
+    const Cols<NV, ODD> cols(threadIdx.x - slot * tpr, tpr, D, off);
+    Feed<NV, ODD, NT> feed;
     feed.t[0] = a.b, feed.t[1] = a.x;
     if constexpr (FULL)
         feed.t[2] = a.g.p;
     feed.buf = smem + static_cast<int64_t>(slot) * stages * NT * pitch;
     feed.bar = bars + slot * MAX_STAGES;
-    feed.R = a.R, feed.D = D, feed.pitch = pitch, feed.stages = stages;
-    const int64_t step = static_cast<int64_t>(gridDim.x) * slots;
-    int64_t row = static_cast<int64_t>(blockIdx.x) * slots + slot;
+    feed.R = a.R, feed.D = D, feed.off = off, feed.pitch = pitch;
     if (lead) {
         for (int s = 0; s < stages; ++s)
             mbar_init(feed.bar + s, 1);
@@ -279,11 +271,11 @@ __global__ void __launch_bounds__(512) fwd_rows_kernel(const Fwd a, int tpr, int
             feed.issue(s, row + s * step);
     const float inv = 1.0f / static_cast<float>(D);
     float w1[E], w2[E];  // w1 with a gate per column folded in
-    cols.load(w1, a.w1, true);
-    cols.load(w2, a.w2, a.w2 != nullptr);
+    cols.template load<false>(w1, a.w1, true);
+    cols.template load<false>(w2, a.w2, a.w2 != nullptr);
     if (a.g.kind == TTK_GATE_COLUMN) {
         float g[E];
-        cols.load(g, a.g.p, true);
+        cols.template load<false>(g, a.g.p, true);
 #pragma unroll
         for (int i = 0; i < E; ++i)
             w1[i] *= g[i];
@@ -330,7 +322,7 @@ __global__ void __launch_bounds__(512) fwd_rows_kernel(const Fwd a, int tpr, int
             x[i] = a.alpha * x[i] + u;  // h
             s[0] += x[i] * x[i];
         }
-        cols.store(a.h + row * D, x);
+        cols.template store<true>(a.h + row * D, x);
         row_sum(s, red[1], slot, tpr, true);
         const float r2 = 1.0f / sqrtf(s[0] * inv + a.eps);
         if (lead) {
@@ -342,16 +334,16 @@ __global__ void __launch_bounds__(512) fwd_rows_kernel(const Fwd a, int tpr, int
 #pragma unroll
             for (int i = 0; i < E; ++i)
                 x[i] *= r2 * w2[i];
-            cols.store(a.y + row * D, x);
+            cols.template store<true>(a.y + row * D, x);
             if (a.split)
                 cols.store_split(a.split + row * D, a.R * D, x);
         }
     }
 }
 
-template <int VEC, int NV, bool FULL>
+template <int NV, bool ODD, bool FULL>
 __global__ void __launch_bounds__(512) bwd_rows_kernel(const Bwd a, int tpr, int pitch, int stages) {
-    constexpr int E = VEC * NV, NT = FULL ? 5 : 4;
+    constexpr int E = 4 * NV, NT = FULL ? 5 : 4;
     extern __shared__ __align__(16) float smem[];
     __shared__ float red[2][3 * MAX_WARPS];
     __shared__ double s_g[MAX_SLOTS];
@@ -359,17 +351,18 @@ __global__ void __launch_bounds__(512) bwd_rows_kernel(const Bwd a, int tpr, int
     const int slot = threadIdx.x / tpr, slots = blockDim.x / tpr;
     const bool lead = threadIdx.x == slot * tpr;
     const int64_t D = a.D;
-    const Cols<VEC, NV> cols(threadIdx.x - slot * tpr, tpr, D);
+    const int64_t step = static_cast<int64_t>(gridDim.x) * slots;
+    int64_t row = static_cast<int64_t>(blockIdx.x) * slots + slot;
+    const int off = ODD ? static_cast<int>((row * D) & 3) : 0;
+    const Cols<NV, ODD> cols(threadIdx.x - slot * tpr, tpr, D, off);
     const bool need_dy = a.dy != nullptr;
-    Feed<VEC, NV, NT> feed;
+    Feed<NV, ODD, NT> feed;
     feed.t[0] = a.dy, feed.t[1] = need_dy ? a.h : nullptr, feed.t[2] = a.dh, feed.t[3] = a.b;
     if constexpr (FULL)
         feed.t[4] = a.g.p;
     feed.buf = smem + static_cast<int64_t>(slot) * stages * NT * pitch;
     feed.bar = bars + slot * MAX_STAGES;
-    feed.R = a.R, feed.D = D, feed.pitch = pitch, feed.stages = stages;
-    const int64_t step = static_cast<int64_t>(gridDim.x) * slots;
-    int64_t row = static_cast<int64_t>(blockIdx.x) * slots + slot;
+    feed.R = a.R, feed.D = D, feed.off = off, feed.pitch = pitch;
     if (lead) {
         for (int s = 0; s < stages; ++s)
             mbar_init(feed.bar + s, 1);
@@ -382,11 +375,11 @@ __global__ void __launch_bounds__(512) bwd_rows_kernel(const Bwd a, int tpr, int
             feed.issue(s, row + s * step);
     const float inv = 1.0f / static_cast<float>(D);
     float w1[E], w2[E];  // w1 with a gate per column folded in
-    cols.load(w1, a.w1, true);
-    cols.load(w2, a.w2, need_dy);
+    cols.template load<false>(w1, a.w1, true);
+    cols.template load<false>(w2, a.w2, need_dy);
     if (a.g.kind == TTK_GATE_COLUMN) {
         float g[E];
-        cols.load(g, a.g.p, true);
+        cols.template load<false>(g, a.g.p, true);
 #pragma unroll
         for (int i = 0; i < E; ++i)
             w1[i] *= g[i];
@@ -471,8 +464,8 @@ __global__ void __launch_bounds__(512) bwd_rows_kernel(const Bwd a, int tpr, int
     if (slots > 1) {
         __syncthreads();
         if (slot) {
-            cols.store(smem + (2 * slot - 2) * D, s1);
-            cols.store(smem + (2 * slot - 1) * D, s2);
+            cols.template store<false>(smem + (2 * slot - 2) * D, s1);
+            cols.template store<false>(smem + (2 * slot - 1) * D, s2);
         }
         if (lead)
             s_g[slot] = gsum;
@@ -480,11 +473,11 @@ __global__ void __launch_bounds__(512) bwd_rows_kernel(const Bwd a, int tpr, int
         if (slot == 0)
             for (int q = 1; q < slots; ++q) {
                 float o[E];
-                cols.load(o, smem + (2 * q - 2) * D, true);
+                cols.template load<false>(o, smem + (2 * q - 2) * D, true);
 #pragma unroll
                 for (int i = 0; i < E; ++i)
                     s1[i] += o[i];
-                cols.load(o, smem + (2 * q - 1) * D, true);
+                cols.template load<false>(o, smem + (2 * q - 1) * D, true);
 #pragma unroll
                 for (int i = 0; i < E; ++i)
                     s2[i] += o[i];
@@ -493,15 +486,16 @@ __global__ void __launch_bounds__(512) bwd_rows_kernel(const Bwd a, int tpr, int
             }
     }
     if (slot == 0) {
-        cols.store(a.part1 + blockIdx.x * D, s1);
-        cols.store(a.part2 + blockIdx.x * D, s2);
+        cols.template store<false>(a.part1 + blockIdx.x * D, s1);
+        cols.template store<false>(a.part2 + blockIdx.x * D, s2);
         if (lead)
             a.partg[blockIdx.x] = gsum;
     }
 }
 
-// Rows too wide for the registers of a block (D > 8192): one block per row,
-// each row read once per pass over it.
+// Rows too wide for the registers of a block (more than 2048 words), or tensors
+// that do not start on a 16-byte boundary: one block per row, each row read once
+// per pass over it.
 constexpr int WIDE_THREADS = 512;
 
 __global__ void __launch_bounds__(WIDE_THREADS) fwd_wide_kernel(const Fwd a) {
@@ -642,11 +636,8 @@ __global__ void __launch_bounds__(32 * FIN_WARPS) finish_kernel(const Bwd a, int
 
 // ----------------------------------------------------------------- launch --
 
-// Threads of a row for `per` words (of 4 floats, or single floats) each.
-int row_threads(int64_t D, int vec, int per) {
-    const int64_t words = (D + vec - 1) / vec;
-    return static_cast<int>(((words + per - 1) / per + 31) / 32 * 32);
-}
+// 16-byte words that a row may touch.
+int64_t row_words(int64_t D) { return D % 4 ? (D + 6) / 4 : D / 4; }
 
 bool aligned16(std::initializer_list<const void*> ps) {
     for (const void* p : ps)
@@ -662,7 +653,7 @@ void partials(Bwd& a, int64_t nb, void* ws) {
     a.partg = reinterpret_cast<double*>(a.part2 + nb * a.D);  // after 2 nb D floats
 }
 
-constexpr int64_t MAX_ROW = 8192;     // widest row kept in registers
+constexpr int64_t MAX_WORDS = 2048;   // widest row kept in registers, in words
 constexpr int64_t MAX_BLOCKS = 2048;  // partial rows of the backward
 constexpr int SMEM_SM = 224 * 1024;   // shared memory of an SM for its blocks' stages
 
@@ -672,16 +663,16 @@ constexpr int SMEM_SM = 224 * 1024;   // shared memory of an SM for its blocks' 
 struct Shape {
     int tpr, slots, threads, pitch, stages;
     size_t smem;
-    int64_t resident;  // blocks
+    int64_t blocks;  // resident at once, or fewer
 };
 
 template <auto kernel>
-Shape shape_of(int64_t R, int64_t D, int vec, int nv, int tensors) {
+Shape shape_of(int64_t R, int64_t D, int nv, int tensors) {
     Shape s;
-    s.tpr = row_threads(D, vec, nv);
+    s.tpr = static_cast<int>(((row_words(D) + nv - 1) / nv + 31) / 32 * 32);
     s.slots = std::max(1, std::min(MAX_SLOTS, 256 / s.tpr));
     s.threads = s.tpr * s.slots;
-    s.pitch = static_cast<int>(vec == 4 ? D : (D + 9) / 4 * 4);  // up to 3 floats at either end
+    s.pitch = static_cast<int>(row_words(D) * 4);
     // {SMs, blocks per SM} by device and block size, asked for once
     constexpr int kDevs = 16;
     static std::atomic<int> cache[kDevs][17];
@@ -712,57 +703,67 @@ Shape shape_of(int64_t R, int64_t D, int vec, int nv, int tensors) {
     s.smem = stage * s.stages;
     while (per > 1 && per * (s.smem + 2048) > SMEM_SM)
         --per;
-    s.resident = static_cast<int64_t>(sms) * per;
+    s.blocks = std::min({(R + s.slots - 1) / s.slots, MAX_BLOCKS, static_cast<int64_t>(sms) * per});
+    // odd widths: the rows of a slot are whole words apart
+    const int64_t apart = D % 4 == 0 ? 1 : D % 2 == 0 ? 2 : 4;
+    while (s.blocks * s.slots < R && s.blocks * s.slots % apart)
+        --s.blocks;
     return s;
 }
 
-template <int VEC, int NV, bool FULL>
+template <int NV, bool ODD, bool FULL>
 int run_fwd(const Fwd& a, cudaStream_t st) {
-    const Shape s = shape_of<fwd_rows_kernel<VEC, NV, FULL>>(a.R, a.D, VEC, NV, FULL ? 3 : 2);
-    const int64_t blocks = std::min((a.R + s.slots - 1) / s.slots, s.resident);
-    return launch_pdl("residual_norm_fwd", fwd_rows_kernel<VEC, NV, FULL>,
-                      dim3(static_cast<unsigned>(blocks)), s.threads, s.smem, st, a, s.tpr, s.pitch,
+    const Shape s = shape_of<fwd_rows_kernel<NV, ODD, FULL>>(a.R, a.D, NV, FULL ? 3 : 2);
+    return launch_pdl("residual_norm_fwd", fwd_rows_kernel<NV, ODD, FULL>,
+                      dim3(static_cast<unsigned>(s.blocks)), s.threads, s.smem, st, a, s.tpr, s.pitch,
                       s.stages);
 }
 
-template <int VEC, int NV, bool FULL>
+template <int NV, bool ODD, bool FULL>
 int run_bwd(Bwd& a, int64_t* nb, void* ws, cudaStream_t st) {
-    const Shape s = shape_of<bwd_rows_kernel<VEC, NV, FULL>>(a.R, a.D, VEC, NV, FULL ? 5 : 4);
-    *nb = std::min({(a.R + s.slots - 1) / s.slots, MAX_BLOCKS, s.resident});
+    const Shape s = shape_of<bwd_rows_kernel<NV, ODD, FULL>>(a.R, a.D, NV, FULL ? 5 : 4);
+    *nb = s.blocks;
     partials(a, *nb, ws);
-    return launch_pdl("residual_norm_bwd", bwd_rows_kernel<VEC, NV, FULL>,
+    return launch_pdl("residual_norm_bwd", bwd_rows_kernel<NV, ODD, FULL>,
                       dim3(static_cast<unsigned>(*nb)), s.threads, s.smem, st, a, s.tpr, s.pitch,
                       s.stages);
 }
 
-int dispatch_fwd(const Fwd& a, bool vec, cudaStream_t st) {
-    const bool full = a.g.kind == TTK_GATE_FULL;
-    if (vec) {
-        if (a.D <= 4096)
-            return full ? run_fwd<4, 2, true>(a, st) : run_fwd<4, 2, false>(a, st);
-        return full ? run_fwd<4, 4, true>(a, st) : run_fwd<4, 4, false>(a, st);
+// `aligned`: every tensor of the rows starts on a 16-byte boundary.
+int dispatch_fwd(const Fwd& a, bool aligned, cudaStream_t st) {
+    const int64_t words = row_words(a.D);
+    if (!aligned || words > MAX_WORDS)
+        return launch_pdl("residual_norm_fwd", fwd_wide_kernel,
+                          dim3(static_cast<unsigned>(grid_for(a.R, 1, 148 * 4))), WIDE_THREADS, 0,
+                          st, a);
+    const bool full = a.g.kind == TTK_GATE_FULL, odd = a.D % 4;
+    if (words <= MAX_WORDS / 2) {
+        if (odd)
+            return full ? run_fwd<2, true, true>(a, st) : run_fwd<2, true, false>(a, st);
+        return full ? run_fwd<2, false, true>(a, st) : run_fwd<2, false, false>(a, st);
     }
-    if (a.D <= 4096)
-        return full ? run_fwd<1, 8, true>(a, st) : run_fwd<1, 8, false>(a, st);
-    return full ? run_fwd<1, 16, true>(a, st) : run_fwd<1, 16, false>(a, st);
+    if (odd)
+        return full ? run_fwd<4, true, true>(a, st) : run_fwd<4, true, false>(a, st);
+    return full ? run_fwd<4, false, true>(a, st) : run_fwd<4, false, false>(a, st);
 }
 
-int dispatch_bwd(Bwd& a, bool vec, int64_t* nb, void* ws, cudaStream_t st) {
-    if (a.D > MAX_ROW) {
+int dispatch_bwd(Bwd& a, bool aligned, int64_t* nb, void* ws, cudaStream_t st) {
+    const int64_t words = row_words(a.D);
+    if (!aligned || words > MAX_WORDS) {
         *nb = std::min<int64_t>(a.R, 296);
         partials(a, *nb, ws);
         return launch_pdl("residual_norm_bwd", bwd_wide_kernel, dim3(static_cast<unsigned>(*nb)),
                           WIDE_THREADS, 0, st, a);
     }
-    const bool full = a.g.kind == TTK_GATE_FULL;
-    if (vec) {
-        if (a.D <= 4096)
-            return full ? run_bwd<4, 2, true>(a, nb, ws, st) : run_bwd<4, 2, false>(a, nb, ws, st);
-        return full ? run_bwd<4, 4, true>(a, nb, ws, st) : run_bwd<4, 4, false>(a, nb, ws, st);
+    const bool full = a.g.kind == TTK_GATE_FULL, odd = a.D % 4;
+    if (words <= MAX_WORDS / 2) {
+        if (odd)
+            return full ? run_bwd<2, true, true>(a, nb, ws, st) : run_bwd<2, true, false>(a, nb, ws, st);
+        return full ? run_bwd<2, false, true>(a, nb, ws, st) : run_bwd<2, false, false>(a, nb, ws, st);
     }
-    if (a.D <= 4096)
-        return full ? run_bwd<1, 8, true>(a, nb, ws, st) : run_bwd<1, 8, false>(a, nb, ws, st);
-    return full ? run_bwd<1, 16, true>(a, nb, ws, st) : run_bwd<1, 16, false>(a, nb, ws, st);
+    if (odd)
+        return full ? run_bwd<4, true, true>(a, nb, ws, st) : run_bwd<4, true, false>(a, nb, ws, st);
+    return full ? run_bwd<4, false, true>(a, nb, ws, st) : run_bwd<4, false, false>(a, nb, ws, st);
 }
 
 }  // namespace resnorm
@@ -801,16 +802,12 @@ int ttk_residual_norm_fwd(const float* x, const float* b, const float* w_post, c
     if (!R)
         return TTK_OK;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    bool vec = D % 4 == 0 && aligned16({x, b, w_post, w_next, h, y});
+    bool aligned = aligned16({x, b, w_post, w_next, h, y});
     if (gate_kind == TTK_GATE_COLUMN || gate_kind == TTK_GATE_FULL)
-        vec = vec && aligned16({gate});
+        aligned = aligned && aligned16({gate});
     const Fwd a{x, b, w_post, Gate{gate, gate_kind}, w_next, h, y, rstd_post, rstd_next,
                 static_cast<__nv_bfloat16*>(y_split), R, D, residual_scale, eps};
-    if (D > MAX_ROW)
-        return launch_pdl("residual_norm_fwd", fwd_wide_kernel,
-                          dim3(static_cast<unsigned>(grid_for(R, 1, 148 * 4))), WIDE_THREADS, 0, st,
-                          a);
-    return dispatch_fwd(a, vec, st);
+    return dispatch_fwd(a, aligned, st);
 }
 
 // Partial rows for any kernel the backward may choose, and one double each.
@@ -844,13 +841,12 @@ int ttk_residual_norm_bwd(const float* dh, const float* dy, const float* h, cons
           nullptr, nullptr, nullptr, accumulate, R, D, residual_scale};
     int64_t nb = 0;
     if (R) {
-        bool vec = D % 4 == 0 && aligned16({dh, dy, b, w_post, dx, db}) &&
-                   (!dy || aligned16({h, w_next}));
+        bool aligned = aligned16({dh, dy, b, w_post, dx, db}) && (!dy || aligned16({h, w_next}));
         if (gate_kind == TTK_GATE_COLUMN)
-            vec = vec && aligned16({gate});
+            aligned = aligned && aligned16({gate});
         if (gate_kind == TTK_GATE_FULL)
-            vec = vec && aligned16({gate, dgate});
-        if (int rc = dispatch_bwd(a, vec, &nb, workspace, st))
+            aligned = aligned && aligned16({gate, dgate});
+        if (int rc = dispatch_bwd(a, aligned, &nb, workspace, st))
             return rc;
     }
     return launch_pdl("residual_norm_bwd sums", finish_kernel,
