@@ -102,6 +102,47 @@ Tensor swiglu(const Tensor& a, const Tensor& b);
 // linear(x, w_up)), w_down) as one op (model.cpp:148-152), same results.
 Tensor ffn_swiglu(const Tensor& x, const Tensor& w_gate, const Tensor& w_up,
                   const Tensor& w_down);
+// ---- operators of a distilled student (extensions; not in the reference) ----
+
+// scale * weight[idx]: [V,D] -> [N,D]; idx -1 (padding) gives a zero row.
+Tensor embedding_scaled(const Tensor& weight, const DeviceIds& idx, float scale);
+
+// One block boundary of a decoder with normalized sub-layer outputs:
+//   h = residual_scale * x + gate * rmsnorm(block, w_post)
+//   y = rmsnorm(h, w_next)
+// x and block [..., D] alike; gate: none (a default Tensor), [1], [D], [R,1]
+// with R = numel / D, or like x. h carries the residual on, y feeds the next
+// block. Both outputs are differentiable; one kernel takes both gradients.
+struct ResidualNorm {
+    Tensor h, y;
+};
+ResidualNorm residual_norm(const Tensor& x, const Tensor& block, const Tensor& w_post,
+                           const Tensor& w_next, const Tensor& gate = Tensor(),
+                           float residual_scale = 1.0f, float eps = 1e-5f);
+
+// A teacher's top logits for n rows on the device: class ids (-1: no entry) and
+// logits, [n, k] each; the logits fp32, bf16 or fp16 (TTK_F32, TTK_BF16,
+// TTK_F16 of ttk.h).
+struct TeacherTop {
+    TeacherTop() = default;
+    TeacherTop(const std::vector<int32_t>& ids, const std::vector<float>& logits, int64_t k);
+    // Adopt device memory (not owned).
+    static TeacherTop borrow(const int32_t* ids, const void* logits, int type, int64_t n,
+                             int64_t k);
+    std::shared_ptr<void> buf;
+    const int32_t* ids = nullptr;
+    const void* logits = nullptr;
+    int type = 0;
+    int64_t n = 0, k = 0;
+};
+// Mean over the rows of alpha T^2 KL(teacher || student at T) + (1 - alpha)
+// cross-entropy(student, targets), the teacher's probabilities taken over its
+// list. targets: ids in [0, C), -1 for a row without a label, or an empty
+// DeviceIds for no labels. parts (or null) receives [3]: the loss, the mean KL
+// and the mean cross-entropy.
+Tensor distill_loss(const Tensor& logits, const TeacherTop& teacher, const DeviceIds& targets,
+                    float alpha, float temperature, Tensor* parts = nullptr);
+
 // Global L2 norm of the gradients of `params`; when max_norm > 0 the
 // gradients are scaled by max_norm / (norm + 1e-6) if that is < 1
 // (the conventional rule; the reference has no clipping). Returns the norm.

@@ -74,3 +74,21 @@ def test_front_end_refusals():
         K.residual_norm_fwd(W, W, W[0], W[0])
     with pytest.raises(ValueError, match="logits: expected"):
         K.distill_loss(W, torch.zeros(4, 2, dtype=torch.int32), torch.zeros(4, 2))
+
+
+def test_programs_compile(tmp_path):
+    """The example and the device test program build against the headers and libraries."""
+    import os
+    import shutil
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    lib = os.path.join(root, "tinytrain_b200", "lib")
+    gxx = shutil.which("g++")
+    if not gxx:
+        pytest.skip("no g++")
+    for src in (("examples", "distill_student.cpp"), ("tests", "cpp", "student_ops.cpp")):
+        r = subprocess.run([gxx, "-std=c++20", "-O1", "-Wall", "-Werror",
+                            "-I" + os.path.join(root, "include"), os.path.join(root, *src),
+                            "-L" + lib, "-ltinytrain", "-lttk", "-Wl,-rpath," + lib, "-o",
+                            str(tmp_path / "prog")], capture_output=True, text=True)
+        assert r.returncode == 0, r.stderr[-3000:]
