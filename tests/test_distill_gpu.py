@@ -320,3 +320,32 @@ def test_rows_at_the_lowest_value(cuda, C):
         ref = torch.stack([0.5 * T * T * kd + 0.5 * ce, kd, ce])
         assert ((loss.double() - ref).abs() <= c * U * (ref + 3)).all()
     assert status() == 0
+
+
+@pytest.mark.parametrize("C", [1000, 3200, 3500, 6000, 10000, 15001, 20000, 40000, 60001])
+@pytest.mark.parametrize("K", [33, 200, 256, 500, 1000])
+def test_long_lists(cuda, C, K):
+    """Long lists leave less room for the row: rows that do not fit beside them."""
+    from tinytrain_b200 import kernels as KN
+    x, ids, top, t, _ = make(9, C, K, cuda)
+    want = define(x, ids, top, t, 0.5, 2.0)
+    check(KN.distill_loss(x, ids, top, t, alpha=0.5, temperature=2.0), want, x, 2.0)
+    check(KN.distill_loss(x, ids, top, t, alpha=0.5, temperature=2.0, want_grad=False), want, x, 2.0)
+
+
+@pytest.mark.parametrize("N,C,K", [(700, 5000, 40), (1300, 700, 12), (2500, 3584, 7), (1200, 3585, 300),
+                                   (900, 12000, 64), (700, 33001, 16), (3000, 17, 5), (1184, 4, 2)])
+def test_many_rows(cuda, N, C, K):
+    """More rows than run at once, with labels, lists and masks of all kinds between them."""
+    from tinytrain_b200 import kernels as KN
+    x, ids, top, t, g = make(N, C, K, cuda)
+    n = torch.randint(0, K + 1, (N, 1), device=cuda, generator=g)
+    ids = torch.where(torch.arange(K, device=cuda) < n, ids, -1).contiguous()
+    t[torch.rand(N, device=cuda, generator=g) < 0.2] = -1
+    w = (torch.rand(N, device=cuda, generator=g) > 0.3).float() * 1.5
+    want = define(x, ids, top, t, 0.7, 2.0, w)
+    out = KN.distill_loss(x, ids, top, t, alpha=0.7, temperature=2.0, row_weight=w)
+    check(out, want, x, 2.0)
+    again = KN.distill_loss(x, ids, top, t, alpha=0.7, temperature=2.0, row_weight=w, dlogits=x)
+    assert torch.equal(again[0], out[0]) and torch.equal(again[1], out[1])
+    assert status() == 0

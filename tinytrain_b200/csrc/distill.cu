@@ -18,7 +18,8 @@
 //     the sums, then the gradient without the teacher's and the label's terms.
 //     A chunk's place is free for the next row's chunk once its gradient is
 //     written, so the copies never pause. Of a row longer than the ring the
-//     last chunks stay, and the others are copied again (from L2);
+//     last chunks stay there and the first in registers; the others are copied
+//     again (from L2);
 //   - a teacher warp works out the next row's list meanwhile, and writes the
 //     listed classes once more after the row, with all their terms.
 // Narrow rows run with fewer compute warps and more CTAs to an SM.
@@ -131,9 +132,9 @@ struct Row {
         chunks = (words + cut.chunk - 1) / cut.chunk;
         keep = a.dlogits ? min(chunks, cut.places) : 0;
     }
-    // copies of the row: every chunk, then those that did not stay
-    __device__ __forceinline__ int copies(const Args& a) const {
-        return a.dlogits ? 2 * chunks - keep : chunks;
+    // chunks that did not stay, the first aside
+    __device__ __forceinline__ int again(const Args& a) const {
+        return a.dlogits ? max(chunks - keep - 1, 0) : 0;
     }
 };
 
@@ -450,10 +451,10 @@ __global__ void __launch_bounds__(32 * (WARPS + 2), CTAS)
                 if (w == 0.0f)
                     continue;
                 const Row r(a, cut, row);
-                const int copies = r.copies(a);
+                const int copies = r.chunks + r.again(a);
                 const float4* src = reinterpret_cast<const float4*>(r.x + r.head);
                 for (int q = 0; q < copies; ++q) {
-                    const int w0 = (q < r.chunks ? q : q - r.chunks) * cut.chunk;
+                    const int w0 = (q < r.chunks ? q : q - r.chunks + 1) * cut.chunk;
                     const uint32_t bytes = static_cast<uint32_t>(min(cut.chunk, r.words - w0)) * 16u;
                     ok = mbar_wait(empty + place, phase ^ 1u, 100);
                     if (!ok)
@@ -543,6 +544,7 @@ __global__ void __launch_bounds__(32 * (WARPS + 2), CTAS)
             }
             const int b = n & 1;
             Stat st = first_stat(x_edge, cT);
+            float4 held[GROUP];  // the first chunk
             int at = place;
             uint32_t ph = phase;
             for (int c = 0; c < r.chunks; ++c) {
@@ -555,7 +557,7 @@ __global__ void __launch_bounds__(32 * (WARPS + 2), CTAS)
                     for (int j = 0; j < GROUP; ++j)
                         v[j] = buf[tid + j * THREADS];
                     push<TWO>(st, v, slack, cT);
-                } else if (tid < words) {
+                } else {
 #pragma unroll
                     for (int j = 0; j < GROUP; ++j)
                         v[j] = tid + j * THREADS < words
@@ -563,6 +565,10 @@ __global__ void __launch_bounds__(32 * (WARPS + 2), CTAS)
                                    : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
                     push<TWO>(st, v, slack, cT);
                 }
+                if (c == 0)
+#pragma unroll
+                    for (int j = 0; j < GROUP; ++j)
+                        held[j] = v[j];
                 if (c < r.chunks - r.keep) {
                     __syncwarp();
                     if (lane == 0)
@@ -585,7 +591,7 @@ __global__ void __launch_bounds__(32 * (WARPS + 2), CTAS)
             if (tid == 0)
                 s_sums[b] = sums;
             if (a.dlogits) {
-                // the chunks that stayed, then the others again
+                // the first chunk, those that stayed, then the others again
                 at = place + (r.chunks - r.keep) % cut.places;
                 ph = phase ^ ((r.chunks - r.keep) / cut.places & 1);
                 if (at >= cut.places)
@@ -593,8 +599,15 @@ __global__ void __launch_bounds__(32 * (WARPS + 2), CTAS)
                 by_kind(sums.kind, same, [&](auto kind, auto aligned) {
                     constexpr int KIND = decltype(kind)::value;
                     constexpr bool ALIGNED = decltype(aligned)::value;
-                    for (int q = r.chunks - r.keep; q < 2 * r.chunks - r.keep; ++q) {
-                        const int w0 = (q < r.chunks ? q : q - r.chunks) * cut.chunk;
+                    if (r.chunks > r.keep && ok) {
+                        float* out = dr + r.head + 4 * tid;
+#pragma unroll
+                        for (int j = 0; j < GROUP; ++j)
+                            if (tid + j * THREADS < cut.chunk)
+                                put<KIND, ALIGNED>(out + 4 * j * THREADS, held[j], sums, cT);
+                    }
+                    for (int q = r.chunks - r.keep; q < r.chunks + r.again(a); ++q) {
+                        const int w0 = (q < r.chunks ? q : q - r.chunks + 1) * cut.chunk;
                         if (q >= r.chunks)
                             ok = ok && mbar_wait(full + at, ph, 105);
                         const float4* buf = ring + at * cut.chunk + tid;
@@ -826,7 +839,7 @@ int launch_rows(const Args& a, cudaStream_t st) {
         return launch<TWO, 2, 4, 8>(a, cut, list_bytes, st);
     if (fits(4) || !a.dlogits)
         return launch<TWO, 4, 6, 4>(a, cut, list_bytes, st);
-    return launch<TWO, 8, 5, 2>(a, cut, list_bytes, st);
+    return launch<TWO, 8, 4, 2>(a, cut, list_bytes, st);
 }
 
 }  // namespace distill
