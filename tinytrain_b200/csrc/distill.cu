@@ -831,10 +831,12 @@ int launch_rows(const Args& a, cudaStream_t st) {
     auto fits = [&](int ctas) {
         return words * 16 * 10 / 14 <= SMEM_SM / ctas - SMEM_CTA - list_bytes;
     };
-    // Few rows: one to a CTA, so as many threads to it as hold it (128 x 32000
-    // without a gradient, kernel alone: 13.6 us with 4 compute warps).
-    if (a.N <= 2 * 148 && a.C > NARROW_MAX)
-        return launch<TWO, 14, 3, 2>(a, cut, list_bytes, st);
+    // Few rows, one to a CTA: the threads of a CTA hold the time down, not the
+    // CTAs of an SM. Measured with 8 warps / as the rules below choose: 128 rows
+    // of 32000 without a gradient 8.7 / 11.3 us, of 8192 with one 8.9 / 11.5 us,
+    // 296 of 32000 10.2 / 12.4 us; 592 of 32000 16.1 / 14.4 us.
+    if (a.N <= 2 * 148)
+        return launch<TWO, 8, 4, 2>(a, cut, list_bytes, st);
     if (fits(8))
         return launch<TWO, 2, 4, 8>(a, cut, list_bytes, st);
     if (fits(4) || !a.dlogits)

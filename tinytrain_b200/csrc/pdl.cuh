@@ -13,11 +13,6 @@ namespace ttk {
 
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-// The next kernel's blocks may take the SMs' free places from here on.
-__device__ __forceinline__ void grid_launch_next() {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-}
-
 template <class... P, class... A>
 int launch_pdl(const char* what, void (*kernel)(P...), dim3 grid, int threads, size_t smem,
                cudaStream_t st, const A&... args) {

@@ -78,17 +78,30 @@ struct Cols {
     static constexpr int E = 4 * NV;
     int w[NV];  // word of the row
     int c[NV];  // its first column (negative in the first word of an odd row)
-    bool in[NV], full[NV];
+    bool in[NV], full[NV], edge;
     int D;
     __device__ __forceinline__ Cols(int t, int tpr, int64_t width, int off)
-        : D(static_cast<int>(width)) {
+        : edge(false), D(static_cast<int>(width)) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             w[j] = j * tpr + t;
             c[j] = 4 * w[j] - (ODD ? off : 0);
             in[j] = c[j] < D;
             full[j] = ODD ? c[j] >= 0 && c[j] + 4 <= D : in[j];
+            edge |= in[j] && !full[j];
         }
+    }
+    // Zeros in place of what the thread's words hold of the neighbouring rows:
+    // one branch for all tensors, which only the two warps at a row's ends take.
+    template <class... V>
+    __device__ __forceinline__ void mask(V&... v) const {
+        if (ODD && edge)
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const int col = c[i / 4] + i % 4;
+                const bool mine = col >= 0 && col < D;
+                ((v[i] = mine ? v[i] : 0.0f), ...);
+            }
     }
     // columns of p, whose alignment is the row's (ALIGNED) or any
     template <bool ALIGNED>
@@ -189,8 +202,8 @@ constexpr int MAX_SLOTS = 8;
 
 // The slot's stages of NT rows (one per tensor; a null tensor is skipped and
 // reads as zeros), `pitch` floats each. A bulk copy moves a row's words whole,
-// with what they hold of its neighbours; the last word of the last row of a
-// tensor has no neighbour behind it and is left to plain loads.
+// with what they hold of its neighbours, which Cols::mask takes out again; the
+// last word of a tensor's last row, if it is not whole, is copied by floats.
 template <int NV, bool ODD, int NT>
 struct Feed {
     static constexpr int E = 4 * NV;
@@ -203,10 +216,13 @@ struct Feed {
     __device__ __forceinline__ void issue(int stage, int64_t row) const {
         uint32_t bytes = static_cast<uint32_t>(D) * 4u;
         if (ODD) {
-            int words = static_cast<int>((off + D + 3) / 4);
-            if (row == R - 1 && (off + D) % 4)
-                --words;
-            bytes = static_cast<uint32_t>(words) * 16u;
+            const int end = static_cast<int>(off + D), tail = row == R - 1 ? end % 4 : 0;
+            bytes = static_cast<uint32_t>((end - tail + 3) / 4) * 16u;
+            if (tail)
+                for (int i = 0; i < NT; ++i)
+                    for (int k = end - tail; k < end; ++k)
+                        if (t[i] && k >= off)
+                            buf[(stage * NT + i) * pitch + k] = t[i][row * D - off + k];
         }
         uint32_t total = 0;
 #pragma unroll
@@ -219,22 +235,13 @@ struct Feed {
                 bulk_load(buf + (stage * NT + i) * pitch, t[i] + row * D - (ODD ? off : 0), bytes,
                           bar + stage);
     }
-    __device__ __forceinline__ void read(float (&v)[E], int i, int stage, int64_t row,
+    __device__ __forceinline__ void read(float (&v)[E], int i, int stage,
                                          const Cols<NV, ODD>& cols) const {
         const float4* b = reinterpret_cast<const float4*>(buf + (stage * NT + i) * pitch);
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const float4 q = t[i] && cols.in[j] ? b[cols.w[j]] : make_float4(0.f, 0.f, 0.f, 0.f);
             v[4 * j] = q.x, v[4 * j + 1] = q.y, v[4 * j + 2] = q.z, v[4 * j + 3] = q.w;
-            if (ODD && t[i] && cols.in[j] && !cols.full[j])  // a word shared with a neighbour
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const int c = cols.c[j] + u;
-                    if (c < 0 || c >= cols.D)
-                        v[4 * j + u] = 0.0f;
-                    else if (row == R - 1)
-                        v[4 * j + u] = t[i][row * D + c];
-                }
         }
     }
 };
@@ -286,10 +293,14 @@ __global__ void __launch_bounds__(512) fwd_rows_kernel(const Fwd a, int tpr, int
         const float gr = a.g.of_row(row);
         bool ok = mbar_wait(feed.bar + stage, phase, 90);
         float x[E], b[E], g[FULL ? E : 1];
-        feed.read(b, 0, stage, row, cols);
-        feed.read(x, 1, stage, row, cols);
+        feed.read(b, 0, stage, cols);
+        feed.read(x, 1, stage, cols);
         if constexpr (FULL)
-            feed.read(g, 2, stage, row, cols);
+            feed.read(g, 2, stage, cols);
+        if constexpr (FULL)
+            cols.mask(b, x, g);
+        else
+            cols.mask(b, x);
         float s[1] = {0.0f};
 #pragma unroll
         for (int i = 0; i < E; ++i)
@@ -395,12 +406,16 @@ __global__ void __launch_bounds__(512) bwd_rows_kernel(const Bwd a, int tpr, int
         const float r1 = a.r1[row], r2 = need_dy ? a.r2[row] : 0.0f, gr = a.g.of_row(row);
         bool ok = mbar_wait(feed.bar + stage, phase, 92);
         float dy[E], h[E], dh[E], b[E], g[FULL ? E : 1];
-        feed.read(dy, 0, stage, row, cols);
-        feed.read(h, 1, stage, row, cols);
-        feed.read(dh, 2, stage, row, cols);
-        feed.read(b, 3, stage, row, cols);
+        feed.read(dy, 0, stage, cols);
+        feed.read(h, 1, stage, cols);
+        feed.read(dh, 2, stage, cols);
+        feed.read(b, 3, stage, cols);
         if constexpr (FULL)
-            feed.read(g, 4, stage, row, cols);
+            feed.read(g, 4, stage, cols);
+        if constexpr (FULL)
+            cols.mask(dy, h, dh, b, g);
+        else
+            cols.mask(dy, h, dh, b);
         float s[3] = {0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < E; ++i) {
