@@ -64,26 +64,35 @@ struct Args {
     int64_t ldd;
 };
 
-// Up to B entries of a lane, 32 apart, of a list from k0 on; none past K.
-template <int B>
-__device__ __forceinline__ void load_top(float (&z)[B], const Args& a, int64_t row, int k0) {
-    const int K = static_cast<int>(a.K), lane = threadIdx.x & 31;
-    const int64_t at = row * a.K + k0 + lane;
-    auto each = [&](auto value) {
+// Up to AHEAD entries of a lane, 32 apart, of a row's list from k0 on (no class past
+// K) and the row's label, as they are in memory: nothing waits for the loads until
+// they are used, so a row's are started while the row before is worked on.
+constexpr int AHEAD = 4;
+struct Entries {
+    int id[AHEAD];
+    uint32_t z[AHEAD];
+    int64_t label;
+    __device__ __forceinline__ void load(const Args& a, int64_t row, int k0) {
+        const int K = row < a.N ? static_cast<int>(a.K) : 0, lane = threadIdx.x & 31;
+        const int64_t at = row * a.K + k0 + lane;
+        label = k0 == 0 && row < a.N && a.targets ? a.targets[row] : -1;
+        const bool wide = a.top_type == TTK_F32;
 #pragma unroll
-        for (int i = 0; i < B; ++i) {
-            z[i] = 0.0f;
-            if (k0 + 32 * i < K && k0 + 32 * i + lane < K)
-                z[i] = value(at + 32 * i);
+        for (int i = 0; i < AHEAD; ++i) {
+            id[i] = -1, z[i] = 0;
+            if (k0 + 32 * i < K && k0 + 32 * i + lane < K) {
+                id[i] = a.ids[at + 32 * i];
+                z[i] = wide ? static_cast<const uint32_t*>(a.top)[at + 32 * i]
+                            : static_cast<const uint16_t*>(a.top)[at + 32 * i];
+            }
         }
-    };
-    if (a.top_type == TTK_F32)
-        each([&](int64_t i) { return static_cast<const float*>(a.top)[i]; });
-    else if (a.top_type == TTK_BF16)
-        each([&](int64_t i) { return __bfloat162float(static_cast<const __nv_bfloat16*>(a.top)[i]); });
-    else
-        each([&](int64_t i) { return __half2float(static_cast<const __half*>(a.top)[i]); });
-}
+    }
+    __device__ __forceinline__ float logit(int i, int type) const {
+        return type == TTK_F32    ? __uint_as_float(z[i])
+               : type == TTK_BF16 ? __uint_as_float(z[i] << 16)
+                                  : __half2float(__ushort_as_half(static_cast<uint16_t>(z[i])));
+    }
+};
 
 // exp((x - m) / T) as a power of two, c = log2 e / T. The difference is taken
 // first: it is exact near the maximum, where the terms that count are, and
@@ -175,90 +184,104 @@ struct Flags {
     bool t_listed;
 };
 
-// Whether a class is in the list more than once, by a hash table of the classes
-// (a single comparison of lanes for up to 32 entries). The same in every lane.
-__device__ __forceinline__ bool listed_twice(const List& l, int K, int* __restrict__ hash, int size) {
+// Whether a class is in the list more than once. Up to 32 entries are compared
+// lane with lane. More go through a table, in rounds: every entry that is
+// still open puts its number into the table at its class's hash and reads what
+// stands there: its own number or that of another entry of its class settle it,
+// and that of another class leaves it open. Entries of one class share a place in
+// every round, so none is missed; a place settles at least the entry that it
+// holds, so the rounds end. The same in every lane.
+__device__ __forceinline__ bool listed_twice(const List& l, int K, int* table, int size) {
     const int lane = threadIdx.x & 31;
     if (K <= 32) {
         const int id = lane < K && l.id[lane] >= 0 ? l.id[lane] : -1 - lane;
         return __any_sync(~0u, __match_any_sync(~0u, id) != 1u << lane);
     }
-    for (int i = lane; i < size; i += 32)
-        hash[i] = -1;
-    __syncwarp();
+    uint32_t open = 0;  // bit i: entry 32 i + lane
+#pragma unroll 4
+    for (int k = lane; k < K; k += 32)
+        if (l.id[k] >= 0)
+            open |= 1u << (k >> 5);
     bool twice = false;
-    for (int k = lane; k < K; k += 32) {
-        const int id = l.id[k];
-        if (id < 0)
-            continue;
-        int h = static_cast<int>((static_cast<unsigned>(id) * 2654435761u) >> 16) & (size - 1);
-        for (int n = 0; n < size; ++n) {
-            const int was = atomicCAS(hash + h, -1, id);
-            twice = twice || was == id;
-            if (was == -1 || was == id)
-                break;
-            h = (h + 1) & (size - 1);
-        }
+    for (uint32_t factor = 2654435761u; __any_sync(~0u, open != 0 && !twice); factor *= 0x9e3779b1u) {
+        auto place = [&](int k) { return (static_cast<uint32_t>(l.id[k]) * factor >> 16) & (size - 1); };
+#pragma unroll 4
+        for (int k = lane; k < K; k += 32)
+            if (open >> (k >> 5) & 1u)
+                table[place(k)] = k;
+        __syncwarp();
+#pragma unroll 4
+        for (int k = lane; k < K; k += 32)
+            if (open >> (k >> 5) & 1u) {
+                const int other = table[place(k)];
+                if (l.id[other] == l.id[k]) {
+                    twice = twice || other != k;
+                    open &= ~(1u << (k >> 5));
+                }
+            }
+        __syncwarp();
     }
     return __any_sync(~0u, twice);
 }
 
-// The teacher warp's work before a row's sums are known. Eight entries of a lane
-// at a time, so that their loads are on the way together; the logits of the
-// first eight are waited for last.
-__device__ void teacher_prepare(const Args& a, const Cut& cut, int64_t row, float w, const List& l,
-                                int* __restrict__ hash, Flags* flags) {
-    constexpr int B = 8;
+// The teacher warp's work before a row's sums are known. `first` holds the row's
+// first entries and, with NEXT, gets those of the row `next`; the student's logits of the
+// first entries are waited for last.
+template <bool NEXT>
+__device__ __forceinline__ void teacher_prepare(const Args& a, const Cut& cut, int64_t row, int64_t next, float w,
+                                const List& l, int* __restrict__ hash, Flags* flags,
+                                Entries& first) {
     const int lane = threadIdx.x & 31, K = static_cast<int>(a.K), C = static_cast<int>(a.C);
     const float invT = 1.0f / a.temperature;
     const float* x = a.logits + row * a.ld;
-    const int64_t label = a.targets ? a.targets[row] : -1;
-    float zmax = -INFINITY, x_first[B];
-    for (int k0 = 0; k0 < K; k0 += 32 * B) {
-        int id[B];
-        float z[B];
+    const int64_t label = first.label;
+    float zmax = -INFINITY, x_first[AHEAD];
+    auto take = [&](const Entries& e, int k0, float (&xs)[AHEAD]) {
 #pragma unroll
-        for (int i = 0; i < B; ++i) {
-            id[i] = -1;
-            if (k0 + 32 * i < K && k0 + 32 * i + lane < K)
-                id[i] = a.ids[row * a.K + k0 + 32 * i + lane];
-        }
-        load_top(z, a, row, k0);
-#pragma unroll
-        for (int i = 0; i < B; ++i) {
+        for (int i = 0; i < AHEAD; ++i) {
             const int k = k0 + 32 * i + lane;
-            float xk = 0.0f;
+            xs[i] = 0.0f;
             if (k0 + 32 * i < K) {
-                if (static_cast<unsigned>(id[i]) >= static_cast<unsigned>(C)) {
-                    if (id[i] != -1)
+                int id = e.id[i];
+                if (static_cast<unsigned>(id) >= static_cast<unsigned>(C)) {
+                    if (id != -1)
                         report(kErrBadIndex);
-                    id[i] = -1;
+                    id = -1;
                 }
-                if (id[i] >= 0)
-                    xk = x[id[i]];
-                const float v = id[i] >= 0 ? z[i] * invT : -INFINITY;
+                if (id >= 0)
+                    xs[i] = x[id];
+                const float v = id >= 0 ? e.logit(i, a.top_type) * invT : -INFINITY;
                 if (k < K) {
-                    l.id[k] = l.to[k] = id[i];
+                    l.id[k] = l.to[k] = id;
                     l.a[k] = v;
                 }
                 // NaN counts as present: it has to reach the row's result
                 zmax = fmaxf(zmax, v != v ? INFINITY : v);
             }
-            if (k0 == 0)
-                x_first[i] = xk;
-            else if (k < K)
-                l.x[k] = xk;
         }
+    };
+    take(first, 0, x_first);
+    for (int k0 = 32 * AHEAD; k0 < K; k0 += 32 * AHEAD) {
+        float xs[AHEAD];
+        first.load(a, row, k0);
+        take(first, k0, xs);
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+            if (k0 + 32 * i + lane < K)
+                l.x[k0 + 32 * i + lane] = xs[i];
     }
     const int t = label >= 0 && label < C ? static_cast<int>(label) : -1;
     if (t < 0 && label != -1 && lane == 0)
         report(kErrBadIndex);
     const float x_t = t >= 0 ? x[t] : 0.0f;
+    if constexpr (NEXT)
+        first.load(a, next, 0);
     zmax = warp_max(zmax);
     const bool has = zmax > -INFINITY;
     __syncwarp();
     float sz = 0.0f;
     bool on_t = false;
+#pragma unroll 4
     for (int k = lane; k < K; k += 32) {
         const float e = has ? expf(l.a[k] - zmax) : 0.0f;
         l.p[k] = e;
@@ -268,12 +291,13 @@ __device__ void teacher_prepare(const Args& a, const Cut& cut, int64_t row, floa
     const bool twice = listed_twice(l, K, hash, cut.hash);
     sz = warp_sum(sz);
     const float logz = logf(sz), invz = 1.0f / sz;
+#pragma unroll 4
     for (int k = lane; k < K; k += 32) {
         l.p[k] = l.sum[k] = has ? l.p[k] * invz : 0.0f;
         l.a[k] = has ? (l.a[k] - zmax) - logz : 0.0f;
     }
 #pragma unroll
-    for (int i = 0; i < B; ++i)
+    for (int i = 0; i < AHEAD; ++i)
         if (32 * i < K && 32 * i + lane < K)
             l.x[32 * i + lane] = x_first[i];
     __syncwarp();
@@ -478,6 +502,8 @@ __global__ void __launch_bounds__(32 * (WARPS + 2), CTAS)
         int64_t before = -1;  // the row before, not finished yet
         int n = 0;
         float w_next = weight_of(a, blockIdx.x);
+        Entries ahead;
+        ahead.load(a, blockIdx.x, 0);
         for (int64_t row = blockIdx.x;; row += gridDim.x) {
             const bool more = row < a.N;
             const float w = w_next;
@@ -485,12 +511,14 @@ __global__ void __launch_bounds__(32 * (WARPS + 2), CTAS)
             const bool work = more && w != 0.0f;
             if (work) {
                 const int b = n & 1;
-                teacher_prepare(a, cut, row, w, List(lists + b * LIST_ARRAYS * pad, pad), hash,
-                                s_flags + b);
+                teacher_prepare<true>(a, cut, row, row + gridDim.x, w,
+                                List(lists + b * LIST_ARRAYS * pad, pad), hash, s_flags + b, ahead);
                 if (lane == 0)
                     mbar_arrive(listed + b);
-            } else if (more && lane == 0) {
-                a.terms[2 * row] = a.terms[2 * row + 1] = 0.0;
+            } else if (more) {
+                ahead.load(a, row + gridDim.x, 0);
+                if (lane == 0)
+                    a.terms[2 * row] = a.terms[2 * row + 1] = 0.0;
             }
             if ((work || !more) && before >= 0) {
                 const int m = n - 1, b = m & 1;
@@ -675,8 +703,10 @@ __global__ void __launch_bounds__(32 * NARROW_WARPS, 8) narrow_kernel(const Args
         const int e = lane < 3 ? (lane < r.head ? lane : -1) : r.head + 4 * r.words + lane - 3;
         const int edge = lane < 6 && e < C ? e : -1;
         const float x_edge = edge >= 0 ? r.x[edge] : -INFINITY;
-        teacher_prepare(a, cut, row, w, l, reinterpret_cast<int*>(mine + LIST_ARRAYS * pad),
-                        s_flags + warp);
+        Entries first;
+        first.load(a, row, 0);
+        teacher_prepare<false>(a, cut, row, 0, w, l,
+                               reinterpret_cast<int*>(mine + LIST_ARRAYS * pad), s_flags + warp, first);
         const Flags f = s_flags[warp];
         Stat st = first_stat(x_edge, cT);
         const float4* x4 = reinterpret_cast<const float4*>(r.x + r.head);
