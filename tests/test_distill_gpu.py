@@ -349,3 +349,19 @@ def test_many_rows(cuda, N, C, K):
     again = KN.distill_loss(x, ids, top, t, alpha=0.7, temperature=2.0, row_weight=w, dlogits=x)
     assert torch.equal(again[0], out[0]) and torch.equal(again[1], out[1])
     assert status() == 0
+
+
+@pytest.mark.parametrize("stride", [1, 64, 128])
+@pytest.mark.parametrize("K", [33, 64, 300])
+@pytest.mark.parametrize("twice", [False, True])
+def test_lists_of_regular_classes(cuda, K, stride, twice):
+    """Classes at a constant stride, whose hashes fall together, all different or
+    with one of them listed a second time at the end."""
+    from tinytrain_b200 import kernels as KN
+    N, C = 5, 128 * 300
+    x, ids, top, t, _ = make(N, C, K, cuda)
+    ids = (torch.arange(K, device=cuda) * stride).int().repeat(N, 1)
+    if twice:
+        ids[:, K - 1] = ids[:, 1]
+    out = KN.distill_loss(x, ids, top, t, alpha=0.5, temperature=2.0)
+    check(out, define(x, ids, top, t, 0.5, 2.0), x, 2.0)

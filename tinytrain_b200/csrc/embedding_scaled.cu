@@ -89,9 +89,10 @@ __global__ void __launch_bounds__(256) lookup_kernel(const float* __restrict__ W
 //     pass. Each warp owns a contiguous run of the pairs: it counts its digits,
 //     the counts are scanned over the warps of the block and over the blocks
 //     (through distributed shared memory), and the warp writes its pairs in
-//     order (24 us for 32768 positions by itself). Up to 65536 positions the pairs stay in the cluster's shared memory
-//     between the passes (LOCAL): through global memory the passes would wait
-//     behind the zeroing blocks' writes.
+//     order (24 us for 32768 positions by itself). Up to 65536 positions the
+//     pairs stay in the cluster's shared memory between the passes (LOCAL):
+//     through global memory the passes would wait behind the zeroing blocks'
+//     writes.
 // Neither needs the whole machine; when dW is written (not added to), the
 // launch's other blocks meanwhile zero the rows of tokens that do not occur.
 // Each owns some of the rows and marks their tokens in a bitmap of its own by

@@ -19,7 +19,12 @@
 // keep it in registers from its one read to its writes. The rows come through
 // shared memory: one thread of the slot copies the slot's next rows with bulk
 // copies, as many ahead as the memory holds, so the reads go on while the
-// slot adds up, waits at its barrier and writes.
+// slot adds up, waits at its barrier and writes. (With plain loads a row ahead
+// in registers instead: 225 and 339 us where this takes 176 and 258.)
+// Measured: 32768 x 2048, gate per column, forward 176 us, 6.1 TB/s, backward
+// 258 us, 6.2 TB/s; backward of 3001 x 1111 with a gate per element 28 us, 3.8
+// TB/s: 7 rows a slot, of which the first load and the last store stand alone
+// (30010 rows: 173 us, 6.2 TB/s).
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -604,7 +609,8 @@ __global__ void __launch_bounds__(WIDE_THREADS) bwd_wide_kernel(const Bwd a) {
 
 // Column sums of the nb partial rows into the weights' and the gate's
 // gradients: 32 columns a block, warp w adds rows w, w + 32, ... and the
-// warps' sums are added in order.
+// warps' sums are added in order. Bound by latency; 8, 16 or 32 columns with 256
+// to 1024 threads, and a tree instead of the last loop, took the same within 1 us.
 constexpr int FIN_WARPS = 32;
 __global__ void __launch_bounds__(32 * FIN_WARPS) finish_kernel(const Bwd a, int64_t nb, float* dw1,
                                                                 float* dw2) {
