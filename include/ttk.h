@@ -399,8 +399,8 @@ int ttk_embedding_scaled_fwd(const float* W, const int64_t* idx, float* out, int
 /* Its gradient by sorted tokens: dW[v,:] = scale * sum of dout[i,:] over the
  * positions i with idx[i] = v (zero rows for tokens that do not occur), or
  * dW += the same with accumulate != 0. Padding and out-of-range ids add
- * nothing. The summation order depends on the ids and on N and D alone: equal
- * calls give equal bits. `workspace` (device, 16-byte aligned) must hold
+ * nothing. The summation order depends on the ids, N, D and whether the rows are
+ * 16-byte aligned alone: equal calls give equal bits. `workspace` (device, 16-byte aligned) must hold
  * ttk_embedding_scaled_bwd_workspace_size(N, D, V) bytes; N and V below 2^31. */
 size_t ttk_embedding_scaled_bwd_workspace_size(int64_t N, int64_t D, int64_t V);
 int ttk_embedding_scaled_bwd(const float* dout, const int64_t* idx, float* dW, int accumulate,
@@ -431,7 +431,8 @@ int ttk_residual_norm_fwd(const float* x, const float* b, const float* w_post, c
  * and dgate in the gate's shape (each of these three may be NULL). `accumulate`
  * is a set of TTK_ACC_* bits: the outputs that are added to instead of
  * written. h, w_next and rstd_next are read only with dy. Outputs must not
- * overlap inputs. The sums over rows are taken in a fixed order. `workspace` (device, 16-byte aligned) must hold
+ * overlap inputs. The sums over rows are taken in a fixed order. `workspace`
+ * (device, 16-byte aligned) must hold
  * ttk_residual_norm_bwd_workspace_size(R, D) bytes. */
 #define TTK_ACC_DX 1
 #define TTK_ACC_DB 2
