@@ -80,11 +80,15 @@ def _gen(seed):
 
 def _tokens(N, V, pad, g):
     """Token ids with the frequencies of text: the id of rank r about as often
-    as 1 / (r + 2.7); with `pad`, the last eighth of each 512 positions is -1."""
-    freq = 1.0 / (torch.arange(V, device="cuda", dtype=torch.float32) + 2.7)
-    ids = torch.multinomial(freq, N, replacement=True, generator=g)
+    as 1 / (r + 2.7); with `pad`, the last eighth of each 512 positions is -1.
+    Looked up in sums made on the host: a parallel prefix sum on the device rounds
+    differently from run to run, and some ids with it."""
+    freq = np.cumsum(1.0 / (np.arange(V) + 2.7))
+    u = torch.rand(N, device=g.device, dtype=torch.float64, generator=g)
+    ids = torch.searchsorted(torch.from_numpy(freq / freq[-1]).to(g.device), u, right=True)
+    ids = ids.clamp(max=V - 1)
     if pad:
-        pos = torch.arange(N, device="cuda") % 512
+        pos = torch.arange(N, device=g.device) % 512
         ids = torch.where(pos >= 448, torch.full_like(ids, -1), ids)
     return ids.contiguous()
 
