@@ -244,11 +244,12 @@ def work(case):
     op = case["op"]
     if op.startswith("embed"):
         N, D, V = case["N"], case["D"], case["V"]
-        if op == "embed_bwd":
-            return {"bytes": 4 * N * D + 4 * V * D + 8 * N, "flops": 2 * N * D}
+        live = N // 512 * 448 + min(N % 512, 448) if case["pad"] else N  # positions with a token
+        if op == "embed_bwd":  # the rows of padding need not be read
+            return {"bytes": 4 * live * D + 4 * V * D + 8 * N, "flops": 2 * live * D}
         r = np.arange(V) + 2.7
-        seen = 1.0 - np.exp(N * np.log1p(-(1.0 / r) / (1.0 / r).sum()))  # expected distinct rows
-        return {"bytes": 4 * N * D + 4 * D * float(seen.sum()) + 8 * N, "flops": N * D}
+        seen = 1.0 - np.exp(live * np.log1p(-(1.0 / r) / (1.0 / r).sum()))  # expected distinct rows
+        return {"bytes": 4 * N * D + 4 * D * float(seen.sum()) + 8 * N, "flops": live * D}
     if op.startswith("norm"):
         n = case["R"] * case["D"]
         full = 4 * n if case["gate"] == "full" else 0
