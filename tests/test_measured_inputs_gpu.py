@@ -46,3 +46,13 @@ def test_token_frequencies(N, V, pad):
     n = int((~padded).sum())
     share = (1 / 2.7) / sum(1 / (r + 2.7) for r in range(V))
     assert abs(int((ids == 0).sum()) - n * share) <= 5 * (n * share * (1 - share)) ** 0.5 + 1
+
+
+@pytest.mark.parametrize("N", [1, 448, 449, 512, 700, 32768])
+def test_padding_is_no_work(N):
+    """A gradient's bytes count the rows of dout that have a token."""
+    D, V = 64, 1000
+    live = sum(i % 512 < 448 for i in range(N))
+    case = dict(op="embed_bwd", N=N, D=D, V=V, pad=True)
+    assert operators.work(case)["bytes"] == 4 * live * D + 4 * V * D + 8 * N
+    assert operators.work(dict(case, pad=False))["bytes"] == 4 * N * D + 4 * V * D + 8 * N
