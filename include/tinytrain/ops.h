@@ -126,7 +126,8 @@ ResidualNorm residual_norm(const Tensor& x, const Tensor& block, const Tensor& w
 struct TeacherTop {
     TeacherTop() = default;
     TeacherTop(const std::vector<int32_t>& ids, const std::vector<float>& logits, int64_t k);
-    // Adopt device memory (not owned).
+    // Adopt device memory (not owned; to be kept, with borrowed targets, until the
+    // last backward of a loss made from it).
     static TeacherTop borrow(const int32_t* ids, const void* logits, int type, int64_t n,
                              int64_t k);
     std::shared_ptr<void> buf;

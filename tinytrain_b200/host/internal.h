@@ -52,6 +52,14 @@ float* grad_rmw(const ImplPtr& p);
 // closure, so a shared_ptr capture would be a cycle and leak the graph.
 const float* grad_in(const Tensor::Impl* p);
 
+// Backward of a scalar loss whose gradient for d(loss) = 1 was made with the loss
+// and is held in `kept`. A gradient of the logits that is still logically zero
+// takes that buffer itself, which from then on belongs to the graph (other nodes
+// hand it on, leaves keep and zero it): `kept` lets go of it, and a later pass over
+// the same graph calls make(d) to write the values again.
+void deliver_loss_grad(const Tensor::Impl* loss, const ImplPtr& logits,
+                       std::shared_ptr<Buffer>& kept, const std::function<void(float*)>& make);
+
 // Scratch device memory released (stream-ordered) when it goes out of scope.
 struct Scratch {
     explicit Scratch(size_t bytes);

@@ -216,38 +216,31 @@ Tensor distill_loss(const Tensor& logits, const TeacherTop& teacher, const Devic
     Tensor all = make_out({3}, false);
     // The gradient for d(loss) = 1 comes with the loss (the rows are read once)
     // and is kept for the backward.
+    auto lo = logits.impl();
+    auto compute = [lo, teacher, targets, N, C, alpha, temperature](float* loss3, float* dlogits) {
+        const size_t ws = ttk_distill_loss_workspace_size(N);
+        Scratch w(ws);
+        check(ttk_distill_loss(dread(lo), C, teacher.ids, teacher.logits, teacher.type, teacher.k,
+                               targets.size() ? targets.data() : nullptr, nullptr, N, C, alpha,
+                               temperature, 1.0f / static_cast<float>(N), loss3, dlogits, C, w.ptr,
+                               ws, stream()),
+              "distill_loss");
+    };
     std::shared_ptr<Buffer> dlog;
     if (logits.requires_grad())
         dlog = std::make_shared<Buffer>(N * C);
-    const size_t ws = ttk_distill_loss_workspace_size(N);
-    Scratch w(ws);
-    check(ttk_distill_loss(dread(logits.impl()), C, teacher.ids, teacher.logits, teacher.type,
-                           teacher.k, targets.size() ? targets.data() : nullptr, nullptr, N, C,
-                           alpha, temperature, 1.0f / static_cast<float>(N), out_ptr(all),
-                           dlog ? dlog->device_for_overwrite() : nullptr, C, w.ptr, ws, stream()),
-          "distill_loss");
+    compute(out_ptr(all), dlog ? dlog->device_for_overwrite() : nullptr);
     check(ttk_memcpy_d2d(out_ptr(out), dread(all.impl()), 4, stream()), "distill_loss");
     if (parts)
         *parts = all;
     if (out.requires_grad()) {
-        auto lo = logits.impl();
         Tensor::Impl* oo = out.impl().get();  // own node: raw, no cycle
         oo->prev = {lo};
-        oo->backward_fn = [lo, oo, dlog, N, C]() {
-            if (!oo->grad || !lo->requires_grad)
-                return;
-            Buffer& og = *oo->grad;
-            const bool unit = og.pending_fill && og.fill_value == 1.0f;
-            if (unit && (!lo->grad || (lo->grad->pending_fill && lo->grad->fill_value == 0.0f &&
-                                       !lo->grad->external)) &&
-                !lo->prev.empty()) {
-                lo->grad = dlog;  // an inner node's: adopted, no copy
-                return;
-            }
-            bool ow = false;
-            float* d = grad_target(lo, ow);
-            check(ttk_axpy_dev(og.device(), dlog->device(), d, N * C, ow ? 0 : 1, stream()),
-                  "distill_loss bwd");
+        oo->backward_fn = [lo, oo, dlog, compute]() mutable {
+            deliver_loss_grad(oo, lo, dlog, [&](float* d) {
+                Scratch loss3(3 * sizeof(float));
+                compute(loss3.as<float>(), d);
+            });
         };
     }
     return out;

@@ -250,6 +250,36 @@ const float* grad_in(const Tensor::Impl* p) {
     return p->grad->device();
 }
 
+void deliver_loss_grad(const Tensor::Impl* loss, const ImplPtr& logits,
+                       std::shared_ptr<Buffer>& kept, const std::function<void(float*)>& make) {
+    if (!loss->grad || !logits->requires_grad)
+        return;
+    if (!kept) {
+        auto again = std::make_shared<Buffer>(logits->numel);
+        make(again->device_for_overwrite());
+        kept = std::move(again);
+    }
+    Buffer& og = *loss->grad;
+    const bool unit = og.pending_fill && og.fill_value == 1.0f;
+    const Buffer* g = logits->grad.get();
+    if (unit && (!g || (g->pending_fill && g->fill_value == 0.0f && !g->external))) {
+        logits->grad = std::move(kept);  // no copy
+        kept.reset();
+        return;
+    }
+    const int64_t n = logits->numel;
+    bool ow = false;
+    float* d = grad_target(logits, ow);
+    if (unit && ow)
+        check(ttk_memcpy_d2d(d, kept->device(), static_cast<size_t>(n) * 4, stream()),
+              "loss grad copy");
+    else if (unit)
+        check(ttk_axpy(1.0f, kept->device(), d, n, stream()), "loss grad");
+    else
+        check(ttk_axpy_dev(og.device(), kept->device(), d, n, ow ? 0 : 1, stream()),
+              "loss grad scale");
+}
+
 }  // namespace detail
 
 // ------------------------------------------------------------------ Tensor --
