@@ -10,7 +10,7 @@ pytestmark = pytest.mark.gpu
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
-@pytest.mark.parametrize("loss", ["distill"])
+@pytest.mark.parametrize("loss", ["distill", "cross_entropy"])
 def test_every_pass_adds_the_same(cuda, tmp_path, loss):
     lib, exe = os.path.join(ROOT, "tinytrain_b200", "lib"), tmp_path / "repeated_backward"
     gxx = shutil.which("g++")

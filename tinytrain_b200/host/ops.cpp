@@ -1024,44 +1024,29 @@ Tensor cross_entropy(const Tensor& logits, const DeviceIds& targets) {
     if (targets.size() != N)
         throw std::invalid_argument("nll_loss: targets size mismatch");
     Tensor out = make_out({1}, logits.requires_grad());
-    Scratch acc(8);
-    check(ttk_memset(acc.ptr, 0, 8, stream()), "ce zero");
     // The gradient for d(loss) = 1 is produced in the same pass (the row is
     // still in registers) and kept for the backward.
+    auto lo = logits.impl();
+    const float inv_n = 1.0f / static_cast<float>(N);
+    auto compute = [lo, targets, N, C, inv_n](double* acc, float* dlogits) {
+        check(ttk_memset(acc, 0, 8, stream()), "ce zero");
+        check(ttk_cross_entropy(dread(lo), targets.data(), N, C, acc, dlogits, inv_n, stream()),
+              "cross_entropy");
+    };
+    Scratch acc(8);
     std::shared_ptr<Buffer> dlog;
     if (logits.requires_grad())
         dlog = std::make_shared<Buffer>(N * C);
-    const float inv_n = 1.0f / static_cast<float>(N);
-    check(ttk_cross_entropy(dread(logits.impl()), targets.data(), N, C, acc.as<double>(),
-                            dlog ? dlog->device_for_overwrite() : nullptr, inv_n, stream()),
-          "cross_entropy");
+    compute(acc.as<double>(), dlog ? dlog->device_for_overwrite() : nullptr);
     check(ttk_loss_finalize(acc.as<double>(), inv_n, out_ptr(out), stream()), "loss");
     if (out.requires_grad()) {
-        auto lo = logits.impl();
         Tensor::Impl* oo = out.impl().get();  // own node: raw, no cycle
         oo->prev = {lo};
-        oo->backward_fn = [lo, oo, dlog, N, C]() {
-            if (!oo->grad || !lo->requires_grad)
-                return;
-            Buffer& og = *oo->grad;
-            const bool unit = og.pending_fill && og.fill_value == 1.0f;
-            if (unit && (!lo->grad || (lo->grad->pending_fill && lo->grad->fill_value == 0.0f))) {
-                lo->grad = dlog;  // adopt the precomputed gradient, no copy
-                return;
-            }
-            bool ow = false;
-            float* d = grad_target(lo, ow);
-            if (unit) {
-                if (ow)
-                    check(ttk_memcpy_d2d(d, dlog->device(), static_cast<size_t>(N * C) * 4,
-                                         stream()),
-                          "ce grad copy");
-                else
-                    check(ttk_axpy(1.0f, dlog->device(), d, N * C, stream()), "ce grad");
-            } else {
-                check(ttk_axpy_dev(og.device(), dlog->device(), d, N * C, ow ? 0 : 1, stream()),
-                      "ce grad scale");
-            }
+        oo->backward_fn = [lo, oo, dlog, compute]() mutable {
+            deliver_loss_grad(oo, lo, dlog, [&](float* d) {
+                Scratch again(8);
+                compute(again.as<double>(), d);
+            });
         };
     }
     return out;
