@@ -1,0 +1,36 @@
+"""Residual norm at its edges: rows narrower than a 16-byte word, whose last words
+lie across the tensors' ends. Bounds as in test_residual_norm_gpu.py."""
+import pytest
+import torch
+
+import test_residual_norm_gpu as base
+
+pytestmark = pytest.mark.gpu
+
+
+def compare(R, D, kind, s, alpha, eps):
+    from tinytrain_b200 import kernels as K
+    h, y, r1, r2 = K.residual_norm_fwd(s["x"], s["b"], s["w1"], s["w2"], gate=s["gate"],
+                                       residual_scale=alpha, eps=eps)
+    h64, hm, y64, ym, _, _ = base.forward64(s, alpha, eps)
+    c = D / 32 + 40
+    base.within(h, h64, hm, c, "h")
+    base.within(y, y64, ym, c, "y")
+    got = K.residual_norm_bwd(s["dh"], s["dy"], h, s["b"], s["w1"], s["w2"], r1, r2,
+                              gate=s["gate"], residual_scale=alpha)
+    ref = list(base.backward64(s, h, r1, r2, alpha, s["dh"], s["dy"]))
+    mag = list(base.backward64(s, h, r1, r2, alpha, s["dh"], s["dy"], positive=True))
+    if s["gate"] is not None:
+        ref[4], mag[4] = base.to_gate(ref[4], s["gate"]), base.to_gate(mag[4], s["gate"])
+    for i, name in enumerate(("dx", "db", "dw_post", "dw_next", "dgate")):
+        if got[i] is not None:
+            rows = R + D if i == 4 and kind == "scalar" else R if i in (2, 3, 4) else 0
+            base.within(got[i].reshape(ref[i].shape), ref[i], mag[i], c + rows, name)
+    assert base.status() == 0
+
+
+@pytest.mark.parametrize("R", [1, 2, 3, 4, 5, 6, 7, 1001, 5003])
+@pytest.mark.parametrize("D", [1, 2, 3, 5])
+@pytest.mark.parametrize("kind", base.GATES)
+def test_narrow_rows(cuda, R, D, kind):
+    compare(R, D, kind, base.make(R, D, kind, cuda), 0.75, 1e-5)

@@ -33,6 +33,7 @@
 #include <initializer_list>
 
 #include "pdl.cuh"
+#include "row_span.h"
 #include "ttk_common.cuh"
 #include "ttk_internal.h"
 
@@ -207,8 +208,8 @@ constexpr int MAX_SLOTS = 8;
 
 // The slot's stages of NT rows (one per tensor; a null tensor is skipped and
 // reads as zeros), `pitch` floats each. A bulk copy moves a row's words whole,
-// with what they hold of its neighbours, which Cols::mask takes out again; the
-// last word of a tensor's last row, if it is not whole, is copied by floats.
+// with what they hold of its neighbours, which Cols::mask takes out again; a word
+// that the tensor's end cuts short is copied by floats (row_span).
 template <int NV, bool ODD, int NT>
 struct Feed {
     static constexpr int E = 4 * NV;
@@ -221,13 +222,12 @@ struct Feed {
     __device__ __forceinline__ void issue(int stage, int64_t row) const {
         uint32_t bytes = static_cast<uint32_t>(D) * 4u;
         if (ODD) {
-            const int end = static_cast<int>(off + D), tail = row == R - 1 ? end % 4 : 0;
-            bytes = static_cast<uint32_t>((end - tail + 3) / 4) * 16u;
-            if (tail)
+            const RowSpan s = row_span(row, R, D, off);
+            bytes = static_cast<uint32_t>(s.words) * 16u;
+            for (int k = 4 * s.words; k < s.end; ++k)
                 for (int i = 0; i < NT; ++i)
-                    for (int k = end - tail; k < end; ++k)
-                        if (t[i] && k >= off)
-                            buf[(stage * NT + i) * pitch + k] = t[i][row * D - off + k];
+                    if (t[i] && k >= off)
+                        buf[(stage * NT + i) * pitch + k] = t[i][row * D - off + k];
         }
         uint32_t total = 0;
 #pragma unroll
