@@ -34,3 +34,22 @@ def compare(R, D, kind, s, alpha, eps):
 @pytest.mark.parametrize("kind", base.GATES)
 def test_narrow_rows(cuda, R, D, kind):
     compare(R, D, kind, base.make(R, D, kind, cuda), 0.75, 1e-5)
+
+
+@pytest.mark.parametrize("kind", base.GATES)
+def test_no_rows(cuda, kind):
+    """Without rows nothing is read: the sums are zero, or what they are added to stays."""
+    from tinytrain_b200 import kernels as K
+    D = 40
+    s = base.make(0, D, kind, cuda)
+    e, r = s["x"], torch.empty(0, device=cuda)
+    args = (e, e, e, e, s["w1"], s["w2"], r, r)
+    _, _, dw1, dw2, dg = K.residual_norm_bwd(*args, gate=s["gate"])
+    assert (dw1 == 0).all() and (dw2 == 0).all() and (dg is None or (dg == 0).all())
+    have = torch.randn(D, device=cuda)
+    keep = None if s["gate"] is None else torch.randn_like(s["gate"])
+    got = K.residual_norm_bwd(*args, gate=s["gate"], dw_post=have.clone(), dw_next=have.clone(),
+                              dgate=None if keep is None else keep.clone())
+    assert torch.equal(got[2], have) and torch.equal(got[3], have)
+    assert keep is None or torch.equal(got[4], keep)
+    assert base.status() == 0

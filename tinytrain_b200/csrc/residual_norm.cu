@@ -793,8 +793,11 @@ int dispatch_bwd(Bwd& a, bool aligned, int64_t* nb, void* ws, cudaStream_t st) {
 using namespace ttk;
 using namespace ttk::resnorm;
 
-static int check_gate(const float* gate, int kind, const char* msg) {
-    if (kind < TTK_GATE_NONE || kind > TTK_GATE_FULL || (kind != TTK_GATE_NONE && !gate))
+// Without rows a gate per row or element has no values, and may be null.
+static int check_gate(const float* gate, int kind, int64_t R, const char* msg) {
+    const bool values = kind == TTK_GATE_SCALAR || kind == TTK_GATE_COLUMN ||
+                        (R && kind != TTK_GATE_NONE);
+    if (kind < TTK_GATE_NONE || kind > TTK_GATE_FULL || (values && !gate))
         return set_error(TTK_ERR_ARG, msg);
     return TTK_OK;
 }
@@ -809,9 +812,8 @@ int ttk_residual_norm_fwd(const float* x, const float* b, const float* w_post, c
         return set_error(TTK_ERR_ARG, "residual_norm_fwd: bad arguments");
     if (R && w_next && (!y || !rstd_next))
         return set_error(TTK_ERR_ARG, "residual_norm_fwd: w_next needs y and rstd_next");
-    if (R)
-        if (int rc = check_gate(gate, gate_kind, "residual_norm_fwd: bad gate"))
-            return rc;
+    if (int rc = check_gate(gate, gate_kind, R, "residual_norm_fwd: bad gate"))
+        return rc;
     if (y_split) {
         if (!w_next || D % 32 || !aligned16({y_split}))
             return set_error(TTK_ERR_ARG, "residual_norm_fwd: planes need w_next, D a multiple of "
@@ -849,27 +851,37 @@ int ttk_residual_norm_bwd(const float* dh, const float* dy, const float* h, cons
         return set_error(TTK_ERR_ARG, "residual_norm_bwd: neither dh nor dy");
     if (R && dy && (!h || !w_next || !rstd_next))
         return set_error(TTK_ERR_ARG, "residual_norm_bwd: dy needs h, w_next and rstd_next");
-    if (R)
-        if (int rc = check_gate(gate, gate_kind, "residual_norm_bwd: bad gate"))
-            return rc;
+    if (int rc = check_gate(gate, gate_kind, R, "residual_norm_bwd: bad gate"))
+        return rc;
     if (accumulate & ~(TTK_ACC_DX | TTK_ACC_DB | TTK_ACC_DW | TTK_ACC_DGATE))
         return set_error(TTK_ERR_ARG, "residual_norm_bwd: unknown accumulate bits");
     if (!workspace || workspace_bytes < ttk_residual_norm_bwd_workspace_size(R, D) ||
         !aligned16({workspace}))
         return set_error(TTK_ERR_ARG, "residual_norm_bwd: workspace too small or not 16-byte aligned");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (!R) {  // sums of nothing: zeros, or what is there
+        auto zero = [&](float* p, int64_t n, int bit) {
+            return !p || !n || (accumulate & bit)
+                       ? TTK_OK
+                       : check_cuda(cudaMemsetAsync(p, 0, static_cast<size_t>(n) * 4, st),
+                                    "residual_norm_bwd: zero");
+        };
+        const int64_t ng = gate_kind == TTK_GATE_SCALAR ? 1 : gate_kind == TTK_GATE_COLUMN ? D : 0;
+        int rc = zero(dw_post, D, TTK_ACC_DW);
+        if (!rc)
+            rc = zero(dw_next, D, TTK_ACC_DW);
+        return rc ? rc : zero(dgate, ng, TTK_ACC_DGATE);
+    }
     Bwd a{dh, dy, h, b, w_post, Gate{gate, gate_kind}, w_next, rstd_post, rstd_next, dx, db, dgate,
           nullptr, nullptr, nullptr, accumulate, R, D, residual_scale};
     int64_t nb = 0;
-    if (R) {
-        bool aligned = aligned16({dh, dy, b, w_post, dx, db}) && (!dy || aligned16({h, w_next}));
-        if (gate_kind == TTK_GATE_COLUMN)
-            aligned = aligned && aligned16({gate});
-        if (gate_kind == TTK_GATE_FULL)
-            aligned = aligned && aligned16({gate, dgate});
-        if (int rc = dispatch_bwd(a, aligned, &nb, workspace, st))
-            return rc;
-    }
+    bool aligned = aligned16({dh, dy, b, w_post, dx, db}) && (!dy || aligned16({h, w_next}));
+    if (gate_kind == TTK_GATE_COLUMN)
+        aligned = aligned && aligned16({gate});
+    if (gate_kind == TTK_GATE_FULL)
+        aligned = aligned && aligned16({gate, dgate});
+    if (int rc = dispatch_bwd(a, aligned, &nb, workspace, st))
+        return rc;
     return launch_pdl("residual_norm_bwd sums", finish_kernel,
                       dim3(static_cast<unsigned>((D + 31) / 32)), 32 * FIN_WARPS, 0, st, a, nb,
                       dw_post, dw_next);
