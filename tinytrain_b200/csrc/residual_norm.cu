@@ -177,8 +177,11 @@ __device__ __forceinline__ bool row_sum(float (&v)[N], float* red, int slot, int
 #pragma unroll
         for (int i = 0; i < N; ++i)
             v[i] += __shfl_xor_sync(~0u, v[i], o);
-    if (tpr == 32)
-        return __all_sync(~0u, ok);
+    if (tpr == 32) {
+        const bool all = __all_sync(~0u, ok);
+        __syncwarp();  // the vote orders no memory: reads of a stage end before its next copy
+        return all;
+    }
     const int warp = threadIdx.x >> 5, w0 = slot * (tpr >> 5), nw = tpr >> 5;
     if ((threadIdx.x & 31) == 0)
 #pragma unroll
