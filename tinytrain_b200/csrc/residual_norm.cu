@@ -227,10 +227,12 @@ struct Feed {
         if (ODD) {
             const RowSpan s = row_span(row, R, D, off);
             bytes = static_cast<uint32_t>(s.words) * 16u;
-            for (int k = 4 * s.words; k < s.end; ++k)
+            if (s.end > 4 * s.words)
+#pragma unroll
                 for (int i = 0; i < NT; ++i)
-                    if (t[i] && k >= off)
-                        buf[(stage * NT + i) * pitch + k] = t[i][row * D - off + k];
+                    for (int k = 4 * s.words; k < s.end; ++k)
+                        if (t[i] && k >= off)
+                            buf[(stage * NT + i) * pitch + k] = t[i][row * D - off + k];
         }
         uint32_t total = 0;
 #pragma unroll
