@@ -53,3 +53,16 @@ def test_no_rows(cuda, kind):
     assert torch.equal(got[2], have) and torch.equal(got[3], have)
     assert keep is None or torch.equal(got[4], keep)
     assert base.status() == 0
+
+
+@pytest.mark.parametrize("size,eps", [(1e14, 1e-5), (1e-14, 0.0), (1e-14, 1e-30)])
+@pytest.mark.parametrize("R,D", [(7, 128), (5, 1111), (3, 8192), (4, 12000)])
+@pytest.mark.parametrize("kind", ["none", "column", "full"])
+def test_sizes_far_from_one(cuda, R, D, kind, size, eps):
+    """Rows of 1e14 or 1e-14: the third power of a row's 1 / rms is no fp32 number, but
+    every output is one."""
+    s = base.make(R, D, kind, cuda)
+    s["x"], s["b"] = s["x"] * size, s["b"] * size
+    if size < 1:  # the residual and the gated norm of b of one size
+        s["w1"] = s["w1"] * size
+    compare(R, D, kind, s, 0.75, eps)

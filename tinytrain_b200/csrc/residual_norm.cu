@@ -10,8 +10,10 @@
 //   dw1 = sum_rows H g b r1,  dw2 = sum_rows dy h r2,  dg = H b r1 w1 summed
 //   to g's shape
 // sum(f b) needs H, which needs sum(e h); with c = g w1 b,
-//   sum(f b) = sum((dh + r2 e) c) - r2^3/D sum(e h) sum(h c),
-// so one round of row sums gives both.
+//   sum(f b) = sum((dh + r2 e) c) - r2^2/D sum(e h) sum(h r2 c),
+// so one round of row sums gives both. A third power of r is taken one factor at a
+// time with the sum it belongs to: by itself it leaves fp32 where a row's values are
+// past 1e13 or below 1e-13.
 //
 // Both directions are bound by HBM: 16 bytes per element forward (x, b in;
 // h, y out), 24 backward (dh, dy, h, b in; dx, db out), 4 or 8 more with a
@@ -435,7 +437,7 @@ __global__ void __launch_bounds__(512) bwd_rows_kernel(const Bwd a, int tpr, int
                 c *= g[i];
             s[0] += e * h[i];
             s[1] += (dh[i] + r2 * e) * c;
-            s[2] += h[i] * c;
+            s[2] += (h[i] * r2) * c;
         }
         ok = row_sum(s, red[parity], slot, tpr, ok);
         if (!ok) {
@@ -454,9 +456,9 @@ __global__ void __launch_bounds__(512) bwd_rows_kernel(const Bwd a, int tpr, int
         }
         if (++stage == stages)
             stage = 0, phase ^= 1;
-        const float k2 = r2 * r2 * r2 * inv * s[0];
-        const float dot = s[1] - k2 * s[2];  // sum(f b) without a gate of the whole row
-        const float k1 = r1 * r1 * r1 * inv * dot * gr, r1g = r1 * gr;
+        const float m2 = r2 * (r2 * (inv * s[0])), k2 = r2 * m2;
+        const float dot = s[1] - m2 * s[2];  // sum(f b) without a gate of the whole row
+        const float k1 = r1 * (r1 * (r1 * (inv * dot))) * gr, r1g = r1 * gr;
         float dx[E], db[E];
         [[maybe_unused]] float dg[FULL ? E : 1];
 #pragma unroll
@@ -581,12 +583,13 @@ __global__ void __launch_bounds__(WIDE_THREADS) bwd_wide_kernel(const Bwd a) {
             const float k = (per_row ? 1.0f : a.g.at(row, c, D)) * a.w1[c] * a.b[o + c];
             s[0] += e * h;
             s[1] += ((a.dh ? a.dh[o + c] : 0.0f) + r2 * e) * k;
-            s[2] += h * k;
+            s[2] += (h * r2) * k;
         }
         row_sum(s, red[parity], 0, WIDE_THREADS, true);
-        const float k2 = r2 * r2 * r2 / static_cast<float>(D) * s[0];
-        const float dot = s[1] - k2 * s[2];
-        const float k1 = r1 * r1 * r1 / static_cast<float>(D) * dot * gr;
+        const float inv = 1.0f / static_cast<float>(D);
+        const float m2 = r2 * (r2 * (inv * s[0])), k2 = r2 * m2;
+        const float dot = s[1] - m2 * s[2];
+        const float k1 = r1 * (r1 * (r1 * (inv * dot))) * gr;
         const bool first = row == blockIdx.x;
         for (int64_t c = threadIdx.x; c < D; c += WIDE_THREADS) {
             const float dy = a.dy ? a.dy[o + c] : 0.0f, h = a.dy ? a.h[o + c] : 0.0f;
