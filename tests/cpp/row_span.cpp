@@ -1,4 +1,4 @@
-// row_span (tinytrain_b200/csrc/row_span.h) for every row of small tensors and the
+// row_tail (tinytrain_b200/csrc/row_span.h) for every row of small tensors and the
 // ends of larger ones: the whole words stay inside the tensor, and with the
 // floats after them they cover the row. Prints "ok" and exits 0 on success.
 #include <cstdio>
@@ -13,12 +13,14 @@ int main() {
             for (int64_t row = R > 16 ? R - 16 : 0; row < R; ++row) {
                 const int off = static_cast<int>(row * D & 3);
                 const int64_t first = row * D - off;  // the first word's first float
-                const ttk::RowSpan s = ttk::row_span(row, R, D, off);
-                const bool inside = s.words >= 0 && first + 4 * s.words <= R * D;
-                const bool covers = s.end == off + D && s.end - 4 * s.words <= 3;
+                const int end = off + static_cast<int>(D);
+                const int tail = ttk::row_tail(row, ttk::first_cut_row(R, D), end);
+                const int words = (end - tail + 3) / 4;  // copied whole
+                const bool inside = words >= 0 && first + 4 * words <= R * D;
+                const bool covers = tail >= 0 && tail <= 3 && 4 * words >= end - tail;
                 if (!inside || !covers) {
                     std::printf("R %lld D %lld row %lld: %d words from %lld, end %d\n", (long long)R,
-                                (long long)D, (long long)row, s.words, (long long)first, s.end);
+                                (long long)D, (long long)row, words, (long long)first, end);
                     ++bad;
                 }
             }

@@ -214,25 +214,24 @@ constexpr int MAX_SLOTS = 8;
 // The slot's stages of NT rows (one per tensor; a null tensor is skipped and
 // reads as zeros), `pitch` floats each. A bulk copy moves a row's words whole,
 // with what they hold of its neighbours, which Cols::mask takes out again; a word
-// that the tensor's end cuts short is copied by floats (row_span).
+// that the tensor's end cuts short is copied by floats (row_tail).
 template <int NV, bool ODD, int NT>
 struct Feed {
     static constexpr int E = 4 * NV;
     const float* t[NT];
     float* buf;  // [stages][NT][pitch]
     uint64_t* bar;
-    int64_t R, D;
+    int64_t first_cut, D;
     int off, pitch;
 
     __device__ __forceinline__ void issue(int stage, int64_t row) const {
         uint32_t bytes = static_cast<uint32_t>(D) * 4u;
         if (ODD) {
-            const RowSpan s = row_span(row, R, D, off);
-            bytes = static_cast<uint32_t>(s.words) * 16u;
-            if (s.end > 4 * s.words)
-#pragma unroll
+            const int end = static_cast<int>(off + D), tail = row_tail(row, first_cut, end);
+            bytes = static_cast<uint32_t>((end - tail + 3) / 4) * 16u;
+            if (tail)
                 for (int i = 0; i < NT; ++i)
-                    for (int k = 4 * s.words; k < s.end; ++k)
+                    for (int k = end - tail; k < end; ++k)
                         if (t[i] && k >= off)
                             buf[(stage * NT + i) * pitch + k] = t[i][row * D - off + k];
         }
@@ -277,7 +276,8 @@ __global__ void __launch_bounds__(512) fwd_rows_kernel(const Fwd a, int tpr, int
         feed.t[2] = a.g.p;
     feed.buf = smem + static_cast<int64_t>(slot) * stages * NT * pitch;
     feed.bar = bars + slot * MAX_STAGES;
-    feed.R = a.R, feed.D = D, feed.off = off, feed.pitch = pitch;
+    feed.first_cut = first_cut_row(a.R, D);
+    feed.D = D, feed.off = off, feed.pitch = pitch;
     if (lead) {
         for (int s = 0; s < stages; ++s)
             mbar_init(feed.bar + s, 1);
@@ -385,7 +385,8 @@ __global__ void __launch_bounds__(512) bwd_rows_kernel(const Bwd a, int tpr, int
         feed.t[4] = a.g.p;
     feed.buf = smem + static_cast<int64_t>(slot) * stages * NT * pitch;
     feed.bar = bars + slot * MAX_STAGES;
-    feed.R = a.R, feed.D = D, feed.off = off, feed.pitch = pitch;
+    feed.first_cut = first_cut_row(a.R, D);
+    feed.D = D, feed.off = off, feed.pitch = pitch;
     if (lead) {
         for (int s = 0; s < stages; ++s)
             mbar_init(feed.bar + s, 1);

@@ -13,19 +13,17 @@
 namespace ttk {
 
 // A row of D floats begins `off` floats into its first word (off = row * D mod 4,
-// the tensor starting on a word). `words` words from that one on are copied whole,
-// with what they hold of the neighbouring rows; the row's floats from 4 * words
-// to its end (at off + D) lie in a word that the tensor's end cuts short (R rows),
-// which no copy of whole words may touch. Rows before the last one can end in
-// that word too: those of width 1.
-struct RowSpan {
-    int words, end;
-};
+// the tensor starting on a word) and ends at off + D. Words are copied whole, with
+// what they hold of the neighbouring rows, but for a word that the tensor's end cuts
+// short, which no such copy may touch.
 
-TTK_HOST_DEVICE RowSpan row_span(int64_t row, int64_t R, int64_t D, int off) {
-    const int end = off + static_cast<int>(D), words = (end + 3) / 4;
-    const bool cut = (R - row) * D + off < 4 * words;  // the tensor ends inside the last word
-    return {cut ? words - 1 : words, end};
+// The first row that may end in that word: the last one, or with width 1 all that
+// share it.
+TTK_HOST_DEVICE int64_t first_cut_row(int64_t R, int64_t D) { return D == 1 ? R - R % 4 : R - 1; }
+
+// How many floats before `end` = off + D lie in it.
+TTK_HOST_DEVICE int row_tail(int64_t row, int64_t first_cut, int end) {
+    return row >= first_cut ? end % 4 : 0;
 }
 
 }  // namespace ttk
