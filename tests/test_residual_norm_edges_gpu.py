@@ -66,3 +66,23 @@ def test_sizes_far_from_one(cuda, R, D, kind, size, eps):
     if size < 1:  # the residual and the gated norm of b of one size
         s["w1"] = s["w1"] * size
     compare(R, D, kind, s, 0.75, eps)
+
+
+def test_sums_over_many_rows(cuda):
+    """The weights' and the gate's gradients over 32768 rows are not one chain of
+    additions. An addition in fp32 is off by about 0.4 u of its result, u = 2^-24, so a
+    chain of n random terms by 0.4 u sqrt(n / 2) of its sum: 16 rows, 7 such sums, 9
+    blocks and 32 of those give 2.3 u together, with the terms' own rounding 2.6 u; one
+    chain of 110 rows in place of the first two would give 3.6 u and more."""
+    from tinytrain_b200 import kernels as K
+    R, D, alpha, eps = 32768, 2048, 0.75, 1e-5
+    s = base.make(R, D, "column", cuda)
+    h, _, r1, r2 = K.residual_norm_fwd(s["x"], s["b"], s["w1"], s["w2"], gate=s["gate"],
+                                       residual_scale=alpha, eps=eps)
+    got = K.residual_norm_bwd(s["dh"], s["dy"], h, s["b"], s["w1"], s["w2"], r1, r2,
+                              gate=s["gate"], residual_scale=alpha)
+    ref = list(base.backward64(s, h, r1, r2, alpha, s["dh"], s["dy"]))
+    ref[4] = base.to_gate(ref[4], s["gate"])
+    for i in (2, 3, 4):
+        err = (got[i].double() - ref[i]).norm() / ref[i].norm()
+        assert err <= 3 * base.U, (i, float(err / base.U))
