@@ -255,7 +255,7 @@ __device__ __forceinline__ void teacher_prepare(const Args& a, const Cut& cut, i
                 }
                 if (id >= 0)
                     xs[i] = x[id];
-                const float v = id >= 0 ? e.logit(i, a.top_type) * invT : -INFINITY;
+                const float v = id >= 0 ? e.logit(i, a.top_type) : -INFINITY;
                 if (k < K) {
                     l.id[k] = l.to[k] = id;
                     l.a[k] = v;
@@ -288,7 +288,11 @@ __device__ __forceinline__ void teacher_prepare(const Args& a, const Cut& cut, i
     bool on_t = false;
 #pragma unroll 4
     for (int k = lane; k < K; k += 32) {
-        const float e = has ? expf(l.a[k] - zmax) : 0.0f;
+        // the difference first, as for the student's logits: z / T may overflow, and
+        // its rounding grows with z (a division by T instead of the product: 202
+        // instead of 185 us at 4096 x 16000 with lists of 250)
+        const float d = has ? (l.a[k] - zmax) * invT : 0.0f, e = has ? expf(d) : 0.0f;
+        l.a[k] = d;
         l.p[k] = e;
         sz += e;
         on_t = on_t || (t >= 0 && l.id[k] == t);
@@ -299,7 +303,7 @@ __device__ __forceinline__ void teacher_prepare(const Args& a, const Cut& cut, i
 #pragma unroll 4
     for (int k = lane; k < K; k += 32) {
         l.p[k] = l.sum[k] = has ? l.p[k] * invz : 0.0f;
-        l.a[k] = has ? (l.a[k] - zmax) - logz : 0.0f;
+        l.a[k] = has ? l.a[k] - logz : 0.0f;
     }
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i)
