@@ -45,3 +45,30 @@ def test_teacher_logits_at_the_types_ends(cuda, N, C, T):
     base.check(out, base.define(x, ids, top, t, 0.5, T), x, T)
     assert torch.isfinite(out[0]).all() and torch.isfinite(out[1]).all()
     assert base.status() == 0
+
+
+@pytest.mark.parametrize("N,C", [(6, 700), (1302, 700), (402, 5000)])
+@pytest.mark.parametrize("T", [1.0, 2.0, 4.0])
+def test_listed_classes_at_the_lowest_value(cuda, N, C, T):
+    """A label or a listed class whose logit is the type's lowest value has a large
+    finite loss, 3.4e38 for the label: a few roundings of the one term that counts."""
+    from tinytrain_b200 import kernels as KN
+    x, ids, top, t, _ = base.make(N, C, 5, cuda)
+    low = torch.finfo(torch.float32).min
+    t = (ids[:, 0].long() + 1) % C
+    x[0, t[0]] = low
+    loss, d = KN.distill_loss(x, ids, top, t, alpha=0.5, temperature=T, grad_scale=0.5)
+    want = base.define(x, ids, top, t, 0.5, T, scale=0.5)[0]
+    assert abs(float(loss[2]) / float(want[2]) - 1) <= 8 * U
+    assert abs(float(loss[0]) / float(want[0]) - 1) <= 8 * U
+    assert abs(float(loss[1]) / float(want[1]) - 1) <= 400 * U
+    x, ids, top, t, _ = base.make(N, C, 5, cuda)
+    x[0, ids[0, 1].long()] = low
+    t[:] = -1
+    loss, d = KN.distill_loss(x, ids, top, t, alpha=1.0, temperature=T, grad_scale=0.125 / T)
+    want = base.define(x, ids, top, t, 1.0, T, scale=0.125 / T)[0]
+    assert float(loss[2]) == 0
+    # p of one entry, with the teacher's exponential and sum around it
+    assert abs(float(loss[0]) / float(want[0]) - 1) <= 60 * U
+    assert torch.isfinite(d).all()
+    assert base.status() == 0

@@ -339,19 +339,20 @@ __device__ void teacher_finish(const Args& a, int64_t row, const List& l, const 
     const int lane = threadIdx.x & 31, K = static_cast<int>(a.K);
     const float w = f.w, gs = a.grad_scale * w;
     const float gT = f.has ? gs * a.alpha * a.temperature : 0.0f;
-    const float g1 = f.t >= 0 ? gs * (1.0f - a.alpha) : 0.0f;
+    const float g1 = f.t >= 0 ? gs * (1.0f - a.alpha) : 0.0f, invT = 1.0f / a.temperature;
     float* dr = a.dlogits + row * a.ldd;
     float kd = 0.0f;
     for (int k = lane; k < K; k += 32) {
         if (l.id[k] >= 0 && l.p[k] != 0.0f)
-            kd += l.p[k] * (l.a[k] - LN2 * ((l.x[k] - r.m) * cT - r.logT));
+            kd += l.p[k] * (l.a[k] - ((l.x[k] - r.m) * invT - LN2 * r.logT));
         if (a.dlogits && write && l.to[k] >= 0)
             dr[l.to[k]] =
                 base_grad(r, l.x[k], cT) - (gT * l.sum[k] + (l.to[k] == f.t ? g1 : 0.0f));
     }
     kd = warp_sum(kd);
     if (lane == 0) {
-        const float ce = f.t >= 0 ? LN2 * (r.log1 - (f.x_t - r.m) * LOG2E) : 0.0f;
+        // not times log2 e and back: a label at the type's lowest value would overflow
+        const float ce = f.t >= 0 ? LN2 * r.log1 - (f.x_t - r.m) : 0.0f;
         if (a.dlogits && write && f.t >= 0 && !f.t_listed)
             dr[f.t] = base_grad(r, f.x_t, cT) - g1;
         a.terms[2 * row] = r.kind ? static_cast<double>(w) * kd : 0.0;
