@@ -622,9 +622,9 @@ int ttk_embedding_scaled_fwd(const float* W, const int64_t* idx, float* out, int
 size_t ttk_embedding_scaled_bwd_workspace_size(int64_t N, int64_t D, int64_t V) {
     if (N <= 0 || D <= 0 || V <= 0)
         return 16;
-    // the scalar form's plan can have shorter chunks than the vector form's
-    const Plan p = plan(N, D, true), q = plan(N, D, false);
-    return std::max(workspace_bytes(p, D), workspace_bytes(q, D));
+    // for either form: the scalar one has as many tiles of the columns or more, so its
+    // chunks are as long or longer, and there are no more of them
+    return workspace_bytes(plan(N, D, true), D);
 }
 
 int ttk_embedding_scaled_bwd(const float* dout, const int64_t* idx, float* dW, int accumulate,
