@@ -86,3 +86,17 @@ def test_sums_over_many_rows(cuda):
     for i in (2, 3, 4):
         err = (got[i].double() - ref[i]).norm() / ref[i].norm()
         assert err <= 3 * base.U, (i, float(err / base.U))
+
+
+def test_gradients_of_nothing(cuda):
+    """A gate's gradient without a gate is refused; w_next's without dy stays as it is."""
+    from tinytrain_b200 import kernels as K
+    R, D = 5, 64
+    s = base.make(R, D, "none", cuda)
+    r1 = torch.ones(R, device=cuda)
+    have = torch.randn(D, device=cuda)
+    with pytest.raises(ValueError, match="dgate: there is no gate"):
+        K.residual_norm_bwd(s["dh"], None, None, s["b"], s["w1"], None, r1, None, dgate=have)
+    got = K.residual_norm_bwd(s["dh"], None, None, s["b"], s["w1"], None, r1, None,
+                              dw_next=have.clone())
+    assert torch.equal(got[3], have)

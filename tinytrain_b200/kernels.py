@@ -236,8 +236,8 @@ def residual_norm_bwd(dh, dy, h, b, w_post, w_next, rstd_post, rstd_next, gate=N
                       residual_scale=1.0, dx=None, db=None, dw_post=None, dw_next=None,
                       dgate=None):
     """(dx, db, dw_post, dw_next, dgate) of residual_norm_fwd; dh or dy may be None (no gradient
-    there). Output tensors that are given are added to; dgate is None without a gate, dw_next
-    without dy."""
+    there). Output tensors that are given are added to; dgate is None without a gate (and refused
+    if given), dw_next without dy (and left as it is if given: nothing is added)."""
     R, D = b.shape
     _chk_all(("dh", "dy", "h", "b", "dx", "db"), (R, D), dh, dy, h, b, dx, db)
     _chk_all(("w_post", "w_next", "dw_post", "dw_next"), (D,), w_post, w_next, dw_post, dw_next)
@@ -261,7 +261,8 @@ def residual_norm_bwd(dh, dy, h, b, w_post, w_next, rstd_post, rstd_next, gate=N
         if dw_next is None and dy is not None:
             dw_next = torch.zeros_like(w_post)
     if gate is None:
-        dgate = None
+        if dgate is not None:
+            raise ValueError("dgate: there is no gate")
     elif dgate is None:
         dgate = torch.empty_like(gate)
     else:
