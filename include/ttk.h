@@ -454,8 +454,8 @@ int ttk_residual_norm_bwd(const float* dh, const float* dy, const float* h, cons
  *   kd = grad_scale * sum_i w_i KD_i,  ce = grad_scale * sum_i w_i CE_i
  *   loss[0..2] = { alpha T^2 kd + (1 - alpha) ce, kd, ce }
  * and, when dlogits is not NULL, dlogits (row stride ldd) is the gradient of
- * loss[0]. dlogits may be logits (with ldd = ld); columns past C are not
- * touched. teacher_logits are of type teacher_type (TTK_F32, TTK_BF16 or
+ * loss[0]. dlogits may be logits (with ldd = ld), and must not overlap it
+ * otherwise; columns past C are not touched. teacher_logits are of type teacher_type (TTK_F32, TTK_BF16 or
  * TTK_F16).
  *   - teacher_ids -1: no entry (a short list); a list without entries, or with
  *     logits of -inf alone, gives no KD part; entries of one class add up

@@ -23,11 +23,12 @@
 //   - a teacher warp works out the next row's list meanwhile, and writes the
 //     listed classes once more after the row, with all their terms.
 // Narrow rows run with fewer compute warps and more CTAs to an SM.
-// Measured: 8192 x 32000 at temperature 2 with lists of 64, loss and gradient, 387
-// us, 5.4 TB/s (365 at temperature 1, with half the exponentials); 1237 x 49999
-// with lists of 50, rows at any alignment, 107 us, 4.6 TB/s (a CTA has 4.2 rows,
-// so the last round leaves most of them idle); loss alone, 4096 x 32000, 98 us,
-// 5.4 TB/s, 128 x 32000 8.8 us.
+// Measured in a CUDA graph, on inputs that are not in L2: 8192 x 32000 at
+// temperature 2 with lists of 64, loss and gradient, 385 us, 5.4 TB/s (386 at
+// temperature 1, with half the exponentials: they are hidden); 1237 x 49999 with
+// lists of 50, rows at any alignment, 107 us, 4.6 TB/s (a CTA has 4.2 rows, so the
+// last round leaves most of them idle); loss alone, 4096 x 32000, 98 us, 5.3 TB/s,
+// 128 x 32000 10.3 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

@@ -6,9 +6,10 @@
 // once, by one summation in a fixed order: no floating-point atomics.
 //
 // Both are bound by HBM. Lookup, 32768 x 2048 of 32000 rows: 57 us, 6.1 TB/s of
-// the rows read and written. Gradient of the same, dW written: 100 us, 5.3 TB/s
-// of dout read and dW written (the sort beside the zeroing of the rows without
-// a token 40, the sums 48, the runs that cross chunks 10).
+// the rows read and written. Gradient of the same with an eighth of padding, dW
+// written: 99 us, 5.0 TB/s of dout read and dW written (kernel by kernel the sort
+// beside the zeroing of the rows without a token 43, the sums 49, the runs that cross
+// chunks 13); added to dW, without padding 118 us.
 #include <cuda_runtime.h>
 #include <stdint.h>
 

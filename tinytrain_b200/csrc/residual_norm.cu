@@ -22,11 +22,13 @@
 // shared memory: one thread of the slot copies the slot's next rows with bulk
 // copies, as many ahead as the memory holds, so the reads go on while the
 // slot adds up, waits at its barrier and writes. (With plain loads a row ahead
-// in registers instead: 225 and 339 us where this takes 176 and 258.)
-// Measured: 32768 x 2048, gate per column, forward 176 us, 6.1 TB/s, backward
-// 258 us, 6.2 TB/s; backward of 3001 x 1111 with a gate per element 28 us, 3.8
-// TB/s: 7 rows a slot, of which the first load and the last store stand alone
-// (30010 rows: 173 us, 6.2 TB/s).
+// in registers instead: 225 and 339 us forward and backward where this took 176
+// and 258, in calls one after the other.)
+// Measured in a CUDA graph, on inputs that are not in L2: 32768 x 2048, gate per
+// column, forward 197 us, 5.4 TB/s (half of it writes), backward 236 us, 6.8 TB/s (a
+// third writes; a copy 6.55); backward of 3001 x 1111 with a gate per element 31 us,
+// 3.4 TB/s: 7 rows a slot, of which the first load and the last store stand alone
+// (30010 rows: 175 us, 6.1 TB/s).
 #include <cuda_runtime.h>
 #include <stdint.h>
 
