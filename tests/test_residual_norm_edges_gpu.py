@@ -100,3 +100,12 @@ def test_gradients_of_nothing(cuda):
     got = K.residual_norm_bwd(s["dh"], None, None, s["b"], s["w1"], None, r1, None,
                               dw_next=have.clone())
     assert torch.equal(got[3], have)
+
+
+@pytest.mark.parametrize("R,D", [(100000, 32), (90000, 66), (80000, 304), (30000, 1111), (20000, 2048),
+                                 (6000, 8190), (5500, 8192)])
+@pytest.mark.parametrize("kind", ["column", "row", "full"])
+def test_slots_of_many_rows(cuda, R, D, kind):
+    """Slots of more than 32 rows, whose sums go through shared memory, in every form of the
+    kernel: several slots a block or one, whole words or not, two or four words a thread."""
+    compare(R, D, kind, base.make(R, D, kind, cuda), 0.75, 1e-5)
